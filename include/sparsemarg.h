@@ -356,6 +356,46 @@ int smlvm_segmented_logsumexp(const float* v, const int64_t* row_offsets, float 
  * then be partly rewritten: discard it). */
 int smlvm_graph_memsets_to_kernels(void* graph /* hipGraph_t */, int32_t* n_memsets, int32_t* n_replaced);
 
+/* ---- operators of a training step next to the hot path -------------------------------------------
+ * No counterpart in the reference, which composes them from torch calls.  Element kinds: */
+#define SMLVM_F32 0
+#define SMLVM_F16 1
+#define SMLVM_BF16 2
+
+/* AdamW over many tensors at once, states in 32 or in 8 bits.  With g the gradient, t = *step + 1:
+ *   m <- beta1 m + (1 - beta1) g;   v <- beta2 v + (1 - beta2) g^2
+ *   p <- p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps);   *step <- t
+ * All arithmetic in fp32 (the 8-bit form's averages in fp64, rounded once to fp32), p rounded to
+ * nearest into its type.
+ * state_bits = 32: m and v are fp32 [n], m_scale / r_scale unused.
+ * state_bits = 8:  m and v point to e4m3 codes [n] (uint8; v's stand for r = sqrt(v)), with one fp32
+ *   scale, a power of two, for every 256 consecutive elements: the smallest 2^k, k >= -100, with
+ *   |x| <= 448 * 2^k over the block's finite elements.  The decoded value is code * scale; p is updated from the
+ *   averages before they are encoded.  Rounding is stochastic, from a counter-based hash of (seed,
+ *   *step + 1, tensor index, element): with q the spacing of e4m3 values at |x| / 2^k and u the low
+ *   (m) or high (r) 16 bits of the hash over 2^16, the code is floor(|x| / 2^k / q + u) q, at most
+ *   448; r > 0 keeps at least the smallest code, so that a denominator never becomes eps alone by
+ *   rounding.  Non-finite values become NaN codes.
+ * `tensors` is a HOST array of `count` entries (read before the call returns).  No two entries may
+ * share memory.  `ticket`: one device word, zero before the first call and left zero; calls that use
+ * one ticket must not overlap.  lr_dev (nullable): the learning rate as a device float, read by the
+ * kernel instead of `lr`. */
+typedef struct {
+    void* p;             /* [n] p_kind, updated in place */
+    const void* g;       /* [n] g_kind */
+    void* m;             /* [n] fp32 / uint8, updated in place */
+    void* v;             /* [n] fp32 / uint8, updated in place */
+    float* m_scale;      /* [ceil(n / 256)] (8-bit states) */
+    float* r_scale;      /* [ceil(n / 256)] (8-bit states) */
+    int64_t* step;       /* device: updates done so far, incremented */
+    int64_t n;
+    uint64_t index;      /* the tensor's number in the rounding hash */
+} smlvm_adamw_tensor;
+int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count, int32_t p_kind, int32_t g_kind,
+                     int32_t state_bits, double beta1, double beta2, float eps, float lr,
+                     const float* lr_dev, float weight_decay, uint32_t seed, uint32_t* ticket,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

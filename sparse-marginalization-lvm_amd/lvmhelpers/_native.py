@@ -6,6 +6,7 @@ wrap the outputs.  There is NO fallback: if the library is missing or a call fai
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -31,6 +32,7 @@ ABI_SYMBOLS = [
     "smlvm_unpack_configs",
     "smlvm_lowrank_ce_fwd", "smlvm_lowrank_ce_fwd_dxdir", "smlvm_lowrank_ce_bwd_workspace_bytes", "smlvm_lowrank_ce_bwd",
     "smlvm_segmented_logsumexp",
+    "smlvm_adamw_step",
 ]
 
 
@@ -746,6 +748,22 @@ def segmented_logsumexp(v, row_offsets, shift=0.0):
         _check(lib().smlvm_segmented_logsumexp(_p(v), _p(row_offsets), _f32(float(shift)), _p(out),
                                                _i64(R), _stream()), "smlvm_segmented_logsumexp")
     return out
+
+
+# ----------------------------------------------------------------------------------- AdamW
+KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # SMLVM_F32, SMLVM_F16, SMLVM_BF16
+ADAMW_ENTRY = struct.Struct("@8QQ")    # smlvm_adamw_tensor: p, g, m, v, m_scale, r_scale, step, n, index
+
+
+def adamw_step(entries, p_dtype, g_dtype, state_bits, betas, eps, lr, weight_decay, seed, ticket):
+    """One smlvm_adamw_step over `entries` (bytes: ADAMW_ENTRY records of tensors on the current
+    device); lr: a number, or a float32 GPU tensor of one element; ticket: int32 [1], zero."""
+    lr_dev = lr if isinstance(lr, torch.Tensor) else None
+    _check(lib().smlvm_adamw_step(
+        ctypes.c_char_p(entries), _i32(len(entries) // ADAMW_ENTRY.size), _i32(KINDS[p_dtype]), _i32(KINDS[g_dtype]),
+        _i32(state_bits), ctypes.c_double(betas[0]), ctypes.c_double(betas[1]), _f32(eps),
+        _f32(0.0 if lr_dev is not None else lr), _p(lr_dev), _f32(weight_decay), ctypes.c_uint32(seed & 0xFFFFFFFF),
+        _p(ticket), _stream()), "smlvm_adamw_step")
 
 
 # ----------------------------------------------------------------------------------- HIP graphs
