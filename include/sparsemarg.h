@@ -396,6 +396,48 @@ int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count, int32_t p
                      const float* lr_dev, float weight_decay, uint32_t seed, uint32_t* ticket,
                      void* stream);
 
+/* Log-probabilities of chosen tokens under softmax(logits) and the entropy of each row:
+ *   logp = z_a - log sum_j exp z_j;   entropy = -sum_j p_j log p_j      (fp32, [B*T])
+ * Row (b, t), 0 <= b < B, 0 <= t < T, starts at logits + b * stride_b + t * stride_t (elements; V
+ * consecutive elements of `kind`, aligned to the element only).  actions [B*T] int64.  -inf logits have probability
+ * 0.  A row without a finite logit, with a NaN or +inf logit or an action outside [0, V) gives NaN.
+ * mask (nullable, [B*T] uint8): rows with 0 are not read; their outputs are 0.
+ * stats [B*T, 3] (nullable): m, s and the entropy, with p_j = exp(z_j - m) / s, for the backward. */
+int smlvm_token_logprobs_fwd(const void* logits, int32_t kind, int64_t stride_b, int64_t stride_t,
+                             const int64_t* actions, const uint8_t* mask, float* logp, float* entropy,
+                             float* stats, int64_t B, int64_t T, int64_t V, void* stream);
+/* Its backward, and the policy loss's: dlogits [B*T, V] contiguous, of `kind`:
+ *   dz_j = g (c (1[j = a] - p_j) - h p_j (log p_j + entropy))
+ * c [B*T] = dL/dlogp, h [B*T] (nullable: 0) = dL/dentropy, g a device float (nullable: 1).  Rows with
+ * mask 0 are written as zeros without being read.  keep_if_one != 0: nothing is written when g is 1
+ * (dlogits then holds the result for g = 1 already, from smlvm_policy_loss). */
+int smlvm_token_logprobs_bwd(const void* logits, int32_t kind, int64_t stride_b, int64_t stride_t,
+                             const int64_t* actions, const uint8_t* mask, const float* stats,
+                             const float* c, const float* h, const float* g, int32_t keep_if_one,
+                             void* dlogits, int64_t B, int64_t T, int64_t V, void* stream);
+
+/* Clipped policy loss with a KL term to a reference policy and an entropy bonus.  Per row, in fp64:
+ *   ratio = exp(logp - old_logp);  d = ref_logp - logp
+ *   l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coeff (e^d - d - 1) - entropy_coeff H
+ *   loss = norm * sum over rows with mask != 0 of l;   norm = mean ? 1 / max(1, #rows with mask != 0) : 1
+ * summed in a fixed order.  logits, actions and mask as above; old_logp, advantages, ref_logp
+ * (nullable: no KL term) fp32 [B*T].
+ * Outputs: loss [1], logp, entropy, kl [B*T] (kl nullable), clipped [B*T] uint8 (1 where the clip is
+ * active; nullable), and for the backward stats [B*T, 3], c = dloss/dlogp [B*T], h = dloss/dentropy
+ * [B*T].  dlogits (nullable) [B*T, V] contiguous: dloss/dlogits, written in the same pass.
+ * workspace: smlvm_policy_loss_workspace_bytes(B*T) bytes, contents ignored. */
+size_t smlvm_policy_loss_workspace_bytes(int64_t rows);
+int smlvm_policy_loss(const void* logits, int32_t kind, int64_t stride_b, int64_t stride_t,
+                      const int64_t* actions, const uint8_t* mask, const float* old_logp,
+                      const float* advantages, const float* ref_logp, float clip_low, float clip_high,
+                      float kl_coeff, float entropy_coeff, int32_t mean, float* loss, float* logp,
+                      float* entropy, float* kl, uint8_t* clipped, float* stats, float* c, float* h,
+                      void* dlogits, int64_t B, int64_t T, int64_t V, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The id of the capture that `stream` is part of, 0 when it is not being captured. */
+int smlvm_stream_capture_id(void* stream, uint64_t* id);
+
 #ifdef __cplusplus
 }
 #endif

@@ -211,13 +211,14 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamwTable table,
         if (whole) store_vec(p_ + at, p); else store_some(p_ + at, have, p);
     }
 
-    // Every workgroup has read its step before it takes a number here; the last one counts all the
-    // launch's tensors up and hands the ticket back at zero.
+    // Every workgroup has read its step before it takes a number here (nothing else is ordered by the
+    // ticket, so it is relaxed: a release would write the whole L2 back); the last one counts all
+    // the launch's tensors up and hands the ticket back at zero.
     __syncthreads();
     if (threadIdx.x == 0) {
-        if (__hip_atomic_fetch_add(hp.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+        if (__hip_atomic_fetch_add(hp.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
             for (int i = 0; i < table.count; ++i) *table.t[i].step += 1;
-            __hip_atomic_store(hp.ticket, 0u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(hp.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
 }

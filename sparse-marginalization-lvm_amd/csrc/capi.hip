@@ -20,3 +20,17 @@ extern "C" const char* smlvm_error_string(int code)
         default: return "unknown error";
     }
 }
+
+extern "C" int smlvm_stream_capture_id(void* stream, uint64_t* id)
+{
+    if (!id) return SMLVM_ERR_INVALID;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long got = 0;
+    const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &got);
+    if (e != hipSuccess) {
+        smlvm::g_last_hip_error = (int)e;
+        return SMLVM_ERR_HIP;
+    }
+    *id = status == hipStreamCaptureStatusActive ? (uint64_t)got : 0;
+    return SMLVM_OK;
+}

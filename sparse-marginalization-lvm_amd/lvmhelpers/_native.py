@@ -33,6 +33,8 @@ ABI_SYMBOLS = [
     "smlvm_lowrank_ce_fwd", "smlvm_lowrank_ce_fwd_dxdir", "smlvm_lowrank_ce_bwd_workspace_bytes", "smlvm_lowrank_ce_bwd",
     "smlvm_segmented_logsumexp",
     "smlvm_adamw_step",
+    "smlvm_token_logprobs_fwd", "smlvm_token_logprobs_bwd", "smlvm_policy_loss_workspace_bytes", "smlvm_policy_loss",
+    "smlvm_stream_capture_id",
 ]
 
 
@@ -64,6 +66,8 @@ def lib():
         L.smlvm_lowrank_ce_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.smlvm_lowrank_ce_bwd_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32,
                                                            ctypes.c_int32, ctypes.c_int32]
+        L.smlvm_policy_loss_workspace_bytes.restype = ctypes.c_size_t
+        L.smlvm_policy_loss_workspace_bytes.argtypes = [ctypes.c_int64]
         if L.smlvm_abi_version() != 2:
             raise NativeError("libsparsemarg_hip.so: ABI version mismatch")
         _lib = L
@@ -120,6 +124,8 @@ def _need_gpu(t, dtype, name):
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     return t.contiguous()
 
+
+KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # SMLVM_F32, SMLVM_F16, SMLVM_BF16
 
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -750,8 +756,88 @@ def segmented_logsumexp(v, row_offsets, shift=0.0):
     return out
 
 
+# ----------------------------------------------------------------------------------- policy loss
+def _need_rows(logits):
+    """logits [B, T, V], one row's elements consecutive (B and T in any stride: a shifted slice of a
+    model's output is read where it lies)."""
+    if not logits.is_cuda:
+        raise NativeError("logits: expected a GPU tensor (the hot path has no CPU fallback)")
+    if logits.dtype not in KINDS:
+        raise TypeError(f"logits: expected float32, float16 or bfloat16, got {logits.dtype}")
+    if logits.shape[2] > 1 and logits.stride(2) != 1:
+        logits = logits.contiguous()
+    return logits
+
+
+def _rows_args(logits, actions, mask):
+    return (_p(logits), _i32(KINDS[logits.dtype]), _i64(logits.stride(0)), _i64(logits.stride(1)), _p(actions), _p(mask))
+
+
+def token_logprobs_fwd(logits, actions, mask=None, want_stats=True):
+    """logits [B,T,V], actions [B,T] int64, mask [B,T] uint8 or None -> (logp, entropy [B,T], stats [B,T,3])."""
+    logits = _need_rows(logits)
+    B, T, V = logits.shape
+    dev = logits.device
+    logp = torch.empty((B, T), dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logp)
+    stats = torch.empty((B, T, 3), dtype=torch.float32, device=dev) if want_stats else None
+    with _on(dev):
+        _check(lib().smlvm_token_logprobs_fwd(*_rows_args(logits, actions, mask), _p(logp), _p(entropy), _p(stats),
+                                              _i64(B), _i64(T), _i64(V), _stream()), "smlvm_token_logprobs_fwd")
+    return logp, entropy, stats
+
+
+def token_logprobs_bwd(logits, actions, mask, stats, c, h, g=None, out=None):
+    """dlogits [B,T,V] = g (c dlogp + h dentropy); out: a buffer that holds the result for g = 1 already
+    (it is written only where g is another number)."""
+    logits = _need_rows(logits)
+    B, T, V = logits.shape
+    keep = out is not None
+    if out is None:
+        out = torch.empty((B, T, V), dtype=logits.dtype, device=logits.device)
+    with _on(logits.device):
+        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), _p(stats), _p(c), _p(h),
+                                              _p(g), _i32(1 if keep else 0), _p(out), _i64(B), _i64(T), _i64(V),
+                                              _stream()), "smlvm_token_logprobs_bwd")
+    return out
+
+
+def policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff, entropy_coeff,
+                mean, want_grad):
+    """-> dict(loss [1], logp, entropy, kl, clipped [B,T], stats [B,T,3], c, h [B,T], dlogits [B,T,V] or None)."""
+    logits = _need_rows(logits)
+    B, T, V = logits.shape
+    dev = logits.device
+    rows = B * T
+    # two allocations for the fp32 outputs (64 rows of a small policy are launch bound): what the caller
+    # gets, and what the backward keeps
+    seen = torch.empty(rows * 3 + 1, dtype=torch.float32, device=dev)
+    kept = torch.empty(rows * 5, dtype=torch.float32, device=dev)
+    out = {k: seen[1 + i * rows:1 + (i + 1) * rows].view(B, T) for i, k in enumerate(("logp", "entropy", "kl"))}
+    out.update(loss=seen[:1], stats=kept[:3 * rows].view(B, T, 3), c=kept[3 * rows:4 * rows].view(B, T),
+               h=kept[4 * rows:].view(B, T))
+    out["clipped"] = torch.empty((B, T), dtype=torch.bool, device=dev)
+    out["dlogits"] = torch.empty((B, T, V), dtype=logits.dtype, device=dev) if want_grad else None
+    nbytes = lib().smlvm_policy_loss_workspace_bytes(rows)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _check(lib().smlvm_policy_loss(
+            *_rows_args(logits, actions, mask), _p(old_logp), _p(advantages), _p(ref_logp), _f32(clip_low),
+            _f32(clip_high), _f32(kl_coeff), _f32(entropy_coeff), _i32(1 if mean else 0), _p(out["loss"]),
+            _p(out["logp"]), _p(out["entropy"]), _p(out["kl"]), _p(out["clipped"]), _p(out["stats"]), _p(out["c"]),
+            _p(out["h"]), _p(out["dlogits"]), _i64(B), _i64(T), _i64(V), _p(ws), ctypes.c_size_t(nbytes), _stream()),
+            "smlvm_policy_loss")
+    return out
+
+
+def capture_id():
+    """The id of the graph capture that the current stream is part of, 0 outside one."""
+    got = ctypes.c_uint64(0)
+    _check(lib().smlvm_stream_capture_id(_stream(), ctypes.byref(got)), "smlvm_stream_capture_id")
+    return got.value
+
+
 # ----------------------------------------------------------------------------------- AdamW
-KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # SMLVM_F32, SMLVM_F16, SMLVM_BF16
 ADAMW_ENTRY = struct.Struct("@8QQ")    # smlvm_adamw_tensor: p, g, m, v, m_scale, r_scale, step, n, index
 
 

@@ -260,6 +260,145 @@ def lowrank_categorical_nll(x, w, b, y):
     return _LowRankCE.apply(x.contiguous(), w.contiguous(), b.contiguous(), y)
 
 
+class _TokenLogprobs(torch.autograd.Function):
+    """(log softmax(logits)[action], entropy) per row without the [.., V] log-probabilities."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, mask):
+        want = ctx.needs_input_grad[0]
+        logp, entropy, stats = _native.token_logprobs_fwd(logits, actions, mask, want_stats=want)
+        if want:
+            ctx.has_mask = mask is not None
+            ctx.save_for_backward(logits, actions, stats, *([mask] if mask is not None else []))
+        return logp, entropy
+
+    @staticmethod
+    def backward(ctx, glogp, gentropy):
+        logits, actions, stats = ctx.saved_tensors[:3]
+        mask = ctx.saved_tensors[3] if ctx.has_mask else None
+        return _native.token_logprobs_bwd(logits, actions, mask, stats, glogp.contiguous(),
+                                          gentropy.contiguous()), None, None
+
+
+class _ClippedPolicyLoss(torch.autograd.Function):
+    """The loss, and in the same pass over the logits its gradient.  The backward hands that buffer on
+    and only launches a kernel that returns at once when the incoming gradient is 1 and writes the
+    gradient anew from the logits when it is not (scaling the stored one would round 16-bit
+    values twice, and lose what fp16 had already flushed to zero).  The buffer is good for one backward
+    pass: a second one (retain_graph), or one recorded into another graph capture than the forward
+    (whose replays need not follow a replay of the forward), computes into a new tensor."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coeff,
+                entropy_coeff, mean):
+        want = ctx.needs_input_grad[0]
+        out = _native.policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff,
+                                  entropy_coeff, mean, want)
+        if want:
+            ctx.has_mask = mask is not None
+            ctx.save_for_backward(logits, actions, out["stats"], out["c"], out["h"],
+                                  *([mask] if mask is not None else []))
+            ctx.ready = out["dlogits"]
+            ctx.capture = _native.capture_id()
+        ctx.mark_non_differentiable(out["logp"], out["entropy"], out["kl"], out["clipped"])
+        return out["loss"].reshape(()), out["logp"], out["entropy"], out["kl"], out["clipped"]
+
+    @staticmethod
+    def backward(ctx, g, *_):
+        logits, actions, stats, c, h = ctx.saved_tensors[:5]
+        mask = ctx.saved_tensors[5] if ctx.has_mask else None
+        ready, ctx.ready = ctx.ready, None
+        if ready is not None and _native.capture_id() != ctx.capture:
+            ready = None
+        dlogits = _native.token_logprobs_bwd(logits, actions, mask, stats, c, h,
+                                             g=g.to(torch.float32).contiguous(), out=ready)
+        return (dlogits,) + (None,) * 10
+
+
+def _policy_rows(logits, actions, name):
+    """logits [..., V] -> [B, T, V] without a copy where the strides allow it, actions -> [B, T] int64."""
+    if logits.dim() < 2 or logits.shape[-1] < 1:
+        raise ValueError(f"{name}: logits must be [..., V] with at least one leading axis and V >= 1")
+    lead = logits.shape[:-1]
+    if tuple(actions.shape) != tuple(lead):
+        raise ValueError(f"{name}: actions must have logits' leading shape {tuple(lead)}, got {tuple(actions.shape)}")
+    if actions.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{name}: actions must be int64 or int32, got {actions.dtype}")
+    if logits.dim() == 2:
+        logits = logits.unsqueeze(0)
+    elif logits.dim() > 3:
+        logits = logits.reshape(-1, logits.shape[-2], logits.shape[-1])
+    return logits, _row_values(actions, lead, logits, name, "actions", torch.int64)
+
+
+def _row_values(t, lead, logits, name, what, dtype):
+    if tuple(t.shape) != tuple(lead):
+        raise ValueError(f"{name}: {what} must have logits' leading shape {tuple(lead)}, got {tuple(t.shape)}")
+    if t.device != logits.device:
+        raise _native.NativeError(f"{name}: {what} must be on the logits' device")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: {what} is a constant of the loss; detach it (no gradient would reach it)")
+    return t.detach().to(dtype).reshape(logits.shape[:2]).contiguous()
+
+
+def _row_mask(mask, lead, logits, name):
+    if mask is None:
+        return None
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"{name}: mask must be bool or uint8, got {mask.dtype}")
+    return _row_values(mask, lead, logits, name, "mask", mask.dtype).view(torch.uint8)
+
+
+def token_logprobs(logits, actions, mask=None):
+    """logits [..., V] (float32, float16, bfloat16), actions [...] integers -> (logp [...], entropy [...]) in
+    float32: the log-probability of each action under softmax(logits) and each row's entropy, without
+    a [..., V] intermediate; differentiable in logits.
+
+    -inf logits have probability zero; a row without a finite logit, with a NaN or +inf one, or with an
+    action outside [0, V) gives NaN.  mask (bool or uint8 [...]): rows that are False are not read and
+    give 0.  Leading axes may be strided (a shifted slice of a model's output is not copied)."""
+    rows, act = _policy_rows(logits, actions, "token_logprobs")
+    lead = logits.shape[:-1]
+    logp, entropy = _TokenLogprobs.apply(rows, act, _row_mask(mask, lead, rows, "token_logprobs"))
+    return logp.view(lead), entropy.view(lead)
+
+
+def clipped_policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None, clip_low=0.2, clip_high=0.2,
+                        kl_coeff=0.0, entropy_coeff=0.0, reduction="mean"):
+    """Clipped policy-gradient loss of a discrete policy, with a KL term to a reference policy and an
+    entropy bonus, straight from the logits:
+
+        ratio = exp(logp - old_logp),   d = ref_logp - logp
+        l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coeff (e^d - d - 1) - entropy_coeff H
+
+    averaged over (reduction="mean") or summed over (="sum") the rows with mask True.
+
+    logits [..., V]; actions, old_logp, advantages, ref_logp, mask [...].  Only logits get a gradient;
+    the others are constants (one that requires a gradient is refused).  Returns (loss, stats) with
+    stats = {'logp', 'entropy', 'kl' (float32), 'clipped' (bool)}, all [...] and without gradient; masked
+    rows are not read, hold zeros there and get a zero gradient.  Other conventions as in `token_logprobs`.
+
+    When logits require a gradient, it is computed in the forward pass (one read of the logits and
+    one write, instead of two reads and one write): memory for it is taken there."""
+    name = "clipped_policy_loss"
+    if reduction not in ("mean", "sum"):
+        raise ValueError(f"{name}: reduction must be 'mean' or 'sum', got {reduction!r}")
+    if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
+        raise ValueError(f"{name}: need 0 <= clip_low <= 1 and clip_high >= 0, got {clip_low}, {clip_high}")
+    if ref_logp is None and kl_coeff != 0.0:
+        raise ValueError(f"{name}: kl_coeff needs ref_logp")
+    rows, act = _policy_rows(logits, actions, name)
+    lead = logits.shape[:-1]
+    f32 = torch.float32
+    old = _row_values(old_logp, lead, rows, name, "old_logp", f32)
+    adv = _row_values(advantages, lead, rows, name, "advantages", f32)
+    ref = None if ref_logp is None else _row_values(ref_logp, lead, rows, name, "ref_logp", f32)
+    loss, logp, entropy, kl, clipped = _ClippedPolicyLoss.apply(
+        rows, act, old, adv, ref, _row_mask(mask, lead, rows, name), float(clip_low), float(clip_high),
+        float(kl_coeff), float(entropy_coeff), reduction == "mean")
+    return loss, {"logp": logp.view(lead), "entropy": entropy.view(lead), "kl": kl.view(lead), "clipped": clipped.view(lead)}
+
+
 _NARROW = (torch.float16, torch.bfloat16)
 
 
