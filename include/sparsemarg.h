@@ -435,6 +435,30 @@ int smlvm_policy_loss(const void* logits, int32_t kind, int64_t stride_b, int64_
                       void* dlogits, int64_t B, int64_t T, int64_t V, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* A linear layer with its epilogue, and its backward.  Element kind `kind` for every matrix and vector:
+ *   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]        x [M, K], w [N, K], y [M, N]
+ *   act: 0 none, 1 relu, 2 gelu (0.5 h (1 + erf(h / sqrt 2))), 3 silu, 4 sigmoid, 5 tanh
+ * Rows of x, w, residual start ldx, ldw, ldr elements apart (elements within a row consecutive); y,
+ * pre, dy, dh, dx, dw contiguous unless a stride is given.  Sums in fp32; 16-bit results are rounded
+ * once.  fp32 operands are split into bf16 parts without loss and multiplied on the bf16 matrix
+ * cores to fp32's accuracy (products below 2^-23 |x||w| are left out); an infinite operand then gives
+ * NaN where fp32 might give an infinity.
+ * bias, residual nullable.  pre (nullable) [M, N]: act's argument, which the backward needs.
+ * workspace: smlvm_linear_workspace_bytes(kind, M, N, K) bytes for any of the three products of one
+ * layer, contents ignored. */
+size_t smlvm_linear_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K);
+int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                     const void* residual, int64_t ldr, void* y, void* pre, int32_t kind, int32_t act,
+                     int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+/* dh = dy act'(h), n elements; h is `pre` (for relu without a residual y does as well). */
+int smlvm_linear_act_bwd(const void* dy, const void* h, void* dh, int32_t kind, int32_t act, int64_t n, void* stream);
+/* dx[m][k] = sum_n dh[m][n] w[n][k] */
+int smlvm_linear_dx(const void* dh, int64_t ldh, const void* w, int64_t ldw, void* dx, int32_t kind, int64_t M,
+                    int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+/* dw[n][k] = sum_m dh[m][n] x[m][k];  db[n] = sum_m dh[m][n] (nullable), from the same pass over dh */
+int smlvm_linear_dw(const void* dh, int64_t ldh, const void* x, int64_t ldx, void* dw, void* db, int32_t kind,
+                    int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The id of the capture that `stream` is part of, 0 when it is not being captured. */
 int smlvm_stream_capture_id(void* stream, uint64_t* id);
 

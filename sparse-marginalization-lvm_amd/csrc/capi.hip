@@ -24,6 +24,8 @@ extern "C" const char* smlvm_error_string(int code)
 extern "C" int smlvm_stream_capture_id(void* stream, uint64_t* id)
 {
     if (!id) return SMLVM_ERR_INVALID;
+    *id = 0;
+    if (!stream) return SMLVM_OK;   // (the default stream is never captured; asking it costs 60 us while it is busy)
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     unsigned long long got = 0;
     const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &got);

@@ -1,0 +1,691 @@
+// Matrix products with a fused epilogue: y = act(x w^T + b) + r, and the two products of its backward
+// (formulas: include/sparsemarg.h).  Compute bound on the matrix cores for many rows, bound by
+// reading w for few.
+//
+// One kernel C[m][n] = sum_k A(m, k) B(n, k) serves all three: an operand is stored either with k
+// consecutive ("rows": x and w in the forward) or with m (n) consecutive ("columns": w in dx = dh w,
+// both in dw = dh^T x).  A row tile is staged as [m][k] and read 16 bytes per lane; a column tile is
+// staged as it lies, [k][m], and transposed by the LDS read (ds_read_b64_tr_b16: 16 lanes read 4 k
+// rows of 16 elements and each receives one column).  Both give a lane 8 consecutive k of one m,
+// the operand layout of v_mfma_f32_16x16x32.  The product is computed as C^T tiles (B first), so that a
+// lane holds 4 consecutive n of one row m and stores them together.
+//
+// 16-bit operands go from memory to LDS directly (buffer_load_dwordx4 ... lds) where rows are aligned to 16
+// bytes, else through registers.  fp32 operands are split exactly into three bf16 parts of 8 bits,
+// x = x1 + x2 + x3 (truncation leaves a remainder of the same sign, 24 bits in all), and the six
+// products of order >= 2^-16 are summed in fp32 on the bf16 matrix cores: what is left out is
+// below 2^-23 of |x||w| per term, the size of fp32's own rounding.  Six bf16 products at 2.5 PFLOP/s
+// are 0.42 PFLOP/s, against 0.157 of the fp32 matrix instructions.
+#include "elements.hpp"
+
+#include <math.h>
+
+namespace smlvm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+#define LDS_PTR(T) __attribute__((address_space(3))) T*
+
+enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5 };
+
+__device__ __forceinline__ float sigmoid_f(float h) { return 1.0f / (1.0f + expf(-h)); }
+
+__device__ __forceinline__ float act_f(int act, float h)
+{
+    switch (act) {
+        case kRelu: return h > 0.0f ? h : (h != h ? h : 0.0f);
+        case kGelu: return 0.5f * h * (1.0f + erff(h * 0.70710678118654752f));
+        case kSilu: return h * sigmoid_f(h);
+        case kSigmoid: return sigmoid_f(h);
+        case kTanh: return tanhf(h);
+        default: return h;
+    }
+}
+__device__ __forceinline__ float act_slope_f(int act, float h)
+{
+    switch (act) {
+        case kRelu: return h > 0.0f ? 1.0f : 0.0f;
+        case kGelu: return 0.5f * (1.0f + erff(h * 0.70710678118654752f)) + h * 0.39894228040143268f * expf(-0.5f * h * h);
+        case kSilu: { const float s = sigmoid_f(h); return s * (1.0f + h * (1.0f - s)); }
+        case kSigmoid: { const float s = sigmoid_f(h); return s * (1.0f - s); }
+        case kTanh: { const float t = tanhf(h); return 1.0f - t * t; }
+        default: return 1.0f;
+    }
+}
+
+struct GemmArgs {
+    const void *a, *b;
+    int64_t lda, ldb;             // elements between rows (k rows of a column operand)
+    int64_t M, N, K;
+    int64_t k_split;              // k range of one blockIdx.z, a multiple of the k tile
+    void* out;                    // [M][N]
+    const void *bias, *res;       // nullable; res [M][N] with row stride ldr
+    int64_t ldr;
+    void* pre;                    // nullable: act's argument [M][N]
+    float* part;                  // not null: fp32 partial sums [splits][M][N] instead of out
+    float* colsum_part;           // not null (column a): fp32 sums over k of A(m, k), [splits][M]
+    int act;
+    int vec;                      // out, pre, res and bias may be accessed 4 elements at a time
+    int tiles_m, tiles_n;
+};
+
+// ----------------------------------------------------------------------------------- epilogue
+template <class T>
+__device__ __forceinline__ void load4(const T* p, bool vec, int have, float (&x)[4])
+{
+    if (vec) {
+        if constexpr (sizeof(T) == 4) load_vec<T, 4>(p, x);
+        else load_vec<T, 4>(p, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = j < have ? (float)p[j] : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, bool vec, int have, const float (&x)[4])
+{
+    if (vec) {
+        store_vec<T, 4>(p, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (j < have) p[j] = (T)x[j];
+    }
+}
+
+// 4 consecutive n of row m: bias, activation, residual, stores
+template <class T>
+__device__ __forceinline__ void finish4(const GemmArgs& g, int64_t m, int64_t n, float (&x)[4])
+{
+    const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
+    const bool vec = g.vec && have == 4;
+    if (g.bias) {
+        float b[4];
+        load4(static_cast<const T*>(g.bias) + n, vec, have, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += b[j];
+    }
+    if (g.pre) store4(static_cast<T*>(g.pre) + m * g.N + n, vec, have, x);
+    if (g.act != kNone) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = act_f(g.act, x[j]);
+    }
+    if (g.res) {
+        float r[4];
+        load4(static_cast<const T*>(g.res) + m * g.ldr + n, vec, have, r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += r[j];
+    }
+    store4(static_cast<T*>(g.out) + m * g.N + n, vec, have, x);
+}
+
+// ------------------------------------------------------------------------------------- staging
+// A tile of ROWS m (n) by BK k.  Row operand in LDS: [ROWS][BK] 16-bit elements, the 16-byte slots of a row
+// exchanged by slot ^ f(row) so that 16 lanes reading one slot of 16 rows touch every bank once;
+// column operand: [BK][ROWS], the 32-byte chunks of a k row exchanged by chunk ^ (k & 7).
+template <int ROWS, int BK, bool COL>
+struct Tile {
+    static constexpr int kBytes = ROWS * BK * 2;
+    static constexpr int kSlots = kBytes / 16;
+    static constexpr int kPerRow = (COL ? ROWS : BK) / 8;               // slots per stored row
+    static constexpr int kMask = COL ? (ROWS / 16 < 8 ? ROWS / 16 : 8) - 1 : kPerRow - 1;
+    static_assert(BK == 32 || BK == 64, "swizzles below");
+
+    // 16-byte slot -> (stored row, first element in it) of the source
+    __device__ __forceinline__ static void source(int slot, int& row, int& at)
+    {
+        row = slot / kPerRow;
+        const int s = slot % kPerRow;
+        if constexpr (COL) at = (((s >> 1) ^ (row & kMask)) << 4) + ((s & 1) << 3);
+        else at = (s ^ ((row / (16 / kPerRow)) & kMask)) << 3;
+    }
+    // lane's 8 k of row `base + lane % 16`, k step kk (of 32): byte offset (row operand)
+    __device__ __forceinline__ static int row_at(int base, int kk, int lane)
+    {
+        const int row = base + (lane & 15), s = kk * 4 + (lane >> 4);
+        return row * (BK * 2) + ((s ^ ((row / (16 / kPerRow)) & kMask)) << 4);
+    }
+    // column operand: p-th (of two) transposing reads
+    __device__ __forceinline__ static int col_at(int base, int kk, int p, int lane)
+    {
+        const int k = kk * 32 + ((lane >> 4) << 3) + p * 4 + ((lane & 15) >> 2);
+        return k * (ROWS * 2) + (((base >> 4) ^ (k & kMask)) << 5) + ((lane & 3) << 3);
+    }
+    __device__ __forceinline__ static s16x8 fragment(const char* tile, int base, int kk, int lane)
+    {
+        if constexpr (COL) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(tile + col_at(base, kk, 0, lane)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(tile + col_at(base, kk, 1, lane)));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const s16x8*>(tile + row_at(base, kk, lane));
+        }
+    }
+};
+
+template <class T>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c)
+{
+    if constexpr (sizeof(T) == 2 && KindOf<T>::value == SMLVM_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from memory to LDS, in flight until the next wait_loads().  The lane's LDS address is
+// `lds` + 16 * lane; offsets beyond the resource's range leave zeros.
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t offset, uint32_t lds)
+{
+    // (4 idle states: the resource may just have been written by a vector instruction; m0 has no other use
+    // in these kernels)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(offset), "s"(rsrc), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void wait_loads_and_sync()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+constexpr uint32_t kOutside = 0x80000000u;                              // = the resource's range
+__device__ __forceinline__ i32x4 resource(const void* p)
+{
+    const uint64_t a = (uint64_t)p;
+    i32x4 r = {__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xFFFF),
+               (int)kOutside, 0x00020000};
+    return r;
+}
+
+// Direct staging of one operand: each thread owns kSlots / THREADS slots, whose offsets into the source
+// (relative to the tile's first row and the current k) never change.
+template <int ROWS, int BK, bool COL, int THREADS>
+struct Direct {
+    using Tl = Tile<ROWS, BK, COL>;
+    static constexpr int kEach = Tl::kSlots / THREADS;
+    static_assert(Tl::kSlots % THREADS == 0, "whole slots per thread");
+    uint32_t offset[kEach];
+    int k_of[kEach];                                                    // k within the tile (slots are all in or all out)
+
+    __device__ __forceinline__ void init(int64_t ld, int64_t first, int64_t extent)
+    {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            int row, at;
+            Tl::source(i * THREADS + threadIdx.x, row, at);
+            k_of[i] = COL ? row : at;
+            const int64_t m = first + (COL ? at : row);
+            offset[i] = m < extent ? (uint32_t)((row * ld + at) * 2) : kOutside;
+        }
+    }
+    // `base`: the tile's first row at the current k
+    __device__ __forceinline__ void issue(const char* base, int64_t k_left, uint32_t lds) const
+    {
+        const i32x4 rsrc = resource(base);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t wave = __builtin_amdgcn_readfirstlane((i * THREADS + (threadIdx.x & ~63)) * 16);
+            load_to_lds(rsrc, k_of[i] < k_left ? offset[i] : kOutside, lds + wave);
+        }
+    }
+};
+
+// Staging through registers: fp32 (split into three planes on the way) and 16-bit operands whose rows are
+// not aligned.
+template <class T, int ROWS, int BK, bool COL, int THREADS>
+struct Through {
+    using Tl = Tile<ROWS, BK, COL>;
+    static constexpr int kEach = Tl::kSlots / THREADS;
+    static constexpr int kVecs = (int)sizeof(T) / 2;                    // 16-byte loads per 8 elements
+    static_assert(Tl::kSlots % THREADS == 0, "whole slots per thread");
+    u32x4 held[kEach][kVecs];
+
+    __device__ __forceinline__ void load(const T* src, int64_t ld, int64_t first, int64_t extent, int64_t k0, int64_t k_end)
+    {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            int row, at;
+            Tl::source(i * THREADS + threadIdx.x, row, at);
+            const int64_t r = COL ? k0 + row : first + row, c = COL ? first + at : k0 + at;
+            const int64_t r_end = COL ? k_end : extent, c_end = COL ? extent : k_end;
+            const T* p = src + r * ld + c;
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) held[i][v] = u32x4{0u, 0u, 0u, 0u};
+            if (r < r_end) {
+                if (c + 8 <= c_end) {
+#pragma unroll
+                    for (int v = 0; v < kVecs; ++v) held[i][v] = reinterpret_cast<const u32x4_any*>(p)[v];
+                } else if (c < c_end) {
+                    T t[8] = {};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) if (c + j < c_end) t[j] = p[j];
+                    __builtin_memcpy(held[i], t, 8 * sizeof(T));
+                }
+            }
+        }
+    }
+    // planes: 1 (16-bit) or 3 (fp32), each a whole tile
+    __device__ __forceinline__ void store(char* tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            char* const to = tile + (i * THREADS + threadIdx.x) * 16;
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<u32x4*>(to) = held[i][0];
+            } else {
+                u32x4 plane[3];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {                            // two elements -> one word of each plane
+                    uint32_t x[2] = {held[i][j >> 1][(j & 1) * 2], held[i][j >> 1][(j & 1) * 2 + 1]};
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        plane[q][j] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302);   // high halves
+                        if (q < 2) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                x[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, x[e]) -
+                                                                        __builtin_bit_cast(float, x[e] & 0xFFFF0000u));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(to + q * Tl::kBytes) = plane[q];
+            }
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------ the kernel
+// BM x BN tile, WM x WN waves, DIRECT: 16-bit aligned operands.
+template <class T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
+{
+    constexpr int THREADS = WM * WN * 64;
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int BK = SPLIT ? 32 : 64;
+    constexpr int PLANES = SPLIT ? 3 : 1;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;                 // 16 x 16 tiles per wave
+    using TA = Tile<BM, BK, ACOL>;
+    using TB = Tile<BN, BK, BCOL>;
+    constexpr int STAGE = PLANES * (TA::kBytes + TB::kBytes);
+    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // Workgroups go round the 8 XCDs: give each XCD, with its own L2, one stretch of tiles, walked in
+    // groups of 8 row tiles so that its neighbours share operands.
+    int id = blockIdx.x;
+    const int tiles = g.tiles_m * g.tiles_n;
+    {
+        const int per = tiles / 8, rest = tiles % 8, xcd = id % 8, at = id / 8;
+        id = xcd * per + (xcd < rest ? xcd : rest) + at;
+    }
+    const int group = id / (8 * g.tiles_n), first_m = group * 8;
+    const int rows_here = g.tiles_m - first_m < 8 ? g.tiles_m - first_m : 8;
+    const int in_group = id - group * 8 * g.tiles_n;
+    const int64_t m0 = (int64_t)(first_m + in_group % rows_here) * BM;
+    const int64_t n0 = (int64_t)(in_group / rows_here) * BN;
+    const int64_t k_begin = (int64_t)blockIdx.z * g.k_split;
+    const int64_t k_end = g.K < k_begin + g.k_split ? g.K : k_begin + g.k_split;
+    const int mw = (wave / WN) * (BM / WM), nw = (wave % WN) * (BN / WN);
+    const bool colsum = ACOL && g.colsum_part && n0 == 0 && wave % WN == 0;
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 sums[ACOL ? FM : 1];
+#pragma unroll
+    for (int i = 0; i < (ACOL ? FM : 1); ++i) sums[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr short kOne = KindOf<T>::value == SMLVM_F16 ? 0x3C00 : 0x3F80;
+    const s16x8 ones = {kOne, kOne, kOne, kOne, kOne, kOne, kOne, kOne};
+
+    auto compute = [&](const char* stage) {
+        const char* const ta = stage;
+        const char* const tb = stage + PLANES * TA::kBytes;
+#pragma unroll
+        for (int kk = 0; kk < BK / 32; ++kk) {
+            s16x8 af[PLANES][FM], bf[PLANES][FN];
+#pragma unroll
+            for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) bf[q][j] = TB::fragment(tb + q * TB::kBytes, nw + j * 16, kk, lane);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) af[q][i] = TA::fragment(ta + q * TA::kBytes, mw + i * 16, kk, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    if constexpr (SPLIT) {                              // smallest terms first
+                        acc[i][j] = mfma<T>(bf[2][j], af[0][i], acc[i][j]);
+                        acc[i][j] = mfma<T>(bf[0][j], af[2][i], acc[i][j]);
+                        acc[i][j] = mfma<T>(bf[1][j], af[1][i], acc[i][j]);
+                        acc[i][j] = mfma<T>(bf[1][j], af[0][i], acc[i][j]);
+                        acc[i][j] = mfma<T>(bf[0][j], af[1][i], acc[i][j]);
+                    }
+                    acc[i][j] = mfma<T>(bf[0][j], af[0][i], acc[i][j]);
+                }
+            if constexpr (ACOL) {
+                if (colsum) {
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int q = PLANES - 1; q >= 0; --q) sums[i] = mfma<T>(ones, af[q][i], sums[i]);
+                }
+            }
+        }
+    };
+
+    const T* const a = static_cast<const T*>(g.a);
+    const T* const b = static_cast<const T*>(g.b);
+    const int64_t steps = k_end > k_begin ? (k_end - k_begin + BK - 1) / BK : 0;
+    if constexpr (DIRECT) {
+        static_assert(!SPLIT, "fp32 goes through registers");
+        Direct<BM, BK, ACOL, THREADS> sa;
+        Direct<BN, BK, BCOL, THREADS> sb;
+        sa.init(g.lda, m0, g.M);
+        sb.init(g.ldb, n0, g.N);
+        const char* pa = reinterpret_cast<const char*>(ACOL ? a + k_begin * g.lda + m0 : a + m0 * g.lda + k_begin);
+        const char* pb = reinterpret_cast<const char*>(BCOL ? b + k_begin * g.ldb + n0 : b + n0 * g.ldb + k_begin);
+        const int64_t ka = (ACOL ? g.lda : 1) * (BK * 2), kb = (BCOL ? g.ldb : 1) * (BK * 2);
+        const uint32_t base = (uint32_t)(uintptr_t)(LDS_PTR(char))lds;
+        auto issue = [&](int64_t step, int buf) {
+            const int64_t left = k_end - k_begin - step * BK;
+            sa.issue(pa + step * ka, left, base + buf * STAGE);
+            sb.issue(pb + step * kb, left, base + buf * STAGE + TA::kBytes);
+        };
+        if (steps > 0) issue(0, 0);
+        for (int64_t s = 0; s < steps; ++s) {
+            // (this tile has arrived, and everybody is done with the buffer that is filled next)
+            wait_loads_and_sync();
+            if (s + 1 < steps) issue(s + 1, (int)((s + 1) & 1));
+            compute(lds + (s & 1) * STAGE);
+        }
+    } else {
+        Through<T, BM, BK, ACOL, THREADS> sa;
+        Through<T, BN, BK, BCOL, THREADS> sb;
+        if (steps > 0) {
+            sa.load(a, g.lda, m0, g.M, k_begin, k_end);
+            sb.load(b, g.ldb, n0, g.N, k_begin, k_end);
+            sa.store(lds);
+            sb.store(lds + PLANES * TA::kBytes);
+        }
+        for (int64_t s = 0; s < steps; ++s) {
+            __syncthreads();
+            if (s + 1 < steps) {
+                sa.load(a, g.lda, m0, g.M, k_begin + (s + 1) * BK, k_end);
+                sb.load(b, g.ldb, n0, g.N, k_begin + (s + 1) * BK, k_end);
+            }
+            compute(lds + (s & 1) * STAGE);
+            if (s + 1 < steps) {
+                char* const to = lds + ((s + 1) & 1) * STAGE;
+                sa.store(to);
+                sb.store(to + PLANES * TA::kBytes);
+            }
+        }
+    }
+
+    const int64_t nb = n0 + nw + ((lane >> 4) << 2), mb = m0 + mw + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t m = mb + i * 16;
+        if (m >= g.M) continue;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int64_t n = nb + j * 16;
+            if (n >= g.N) continue;
+            float x[4] = {acc[i][j].x, acc[i][j].y, acc[i][j].z, acc[i][j].w};
+            if (g.part) {
+                const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
+                store4(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N % 4 == 0, have, x);
+            } else {
+                finish4<T>(g, m, n, x);
+            }
+        }
+        if constexpr (ACOL) {
+            if (colsum && lane < 16) g.colsum_part[(int64_t)blockIdx.z * g.M + m] = sums[i].x;
+        }
+    }
+}
+
+// Joins the partial sums of a split product, in order, and runs the epilogue.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits)
+{
+    const int64_t per_row = (g.N + 3) / 4, total = g.M * per_row;
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+        const int64_t m = v / per_row, n = (v - m * per_row) * 4;
+        const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int z = 0; z < splits; ++z) {
+            float y[4];
+            load4<float>(g.part + ((int64_t)z * g.M + m) * g.N + n, g.N % 4 == 0, have, y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += y[j];
+        }
+        finish4<T>(g, m, n, x);
+    }
+}
+
+// Column sums: db[m] = sum over the splits.
+template <class T>
+__global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict__ part, int splits, int64_t M, T* __restrict__ out)
+{
+    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (m >= M) return;
+    float s = 0.0f;
+    for (int z = 0; z < splits; ++z) s += part[(int64_t)z * M + m];
+    out[m] = (T)s;
+}
+
+// dh = dy act'(h); relu may be given y in the place of h (the sign is the same).
+template <class T>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ h, T* __restrict__ dh,
+                                                      int64_t n, int act, int aligned)
+{
+    const int64_t stride = (int64_t)gridDim.x * 256 * 8;
+    for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < n; at += stride) {
+        float x[8], y[8];
+        if (aligned && at + 8 <= n) {
+            load_vec<T, 8>(h + at, x);
+            load_vec<T, 8>(dy + at, y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= act_slope_f(act, x[j]);
+            store_vec<T, 8>(dh + at, y);
+        } else {
+            for (int j = 0; j < 8 && at + j < n; ++j) dh[at + j] = (T)((float)dy[at + j] * act_slope_f(act, (float)h[at + j]));
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------- host side
+struct Plan { int bm, bn, splits; int64_t k_split; };
+
+// Tile and split: the largest tile that still gives every CU a workgroup; the smallest one otherwise,
+// with the k range split until there are some two workgroups per CU (each keeping 4 k tiles).
+static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
+{
+    const int64_t bk = kind == SMLVM_F32 ? 32 : 64;
+    auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    Plan p = {64, 64, 1, 0};
+    if (direct && tiles(256) >= 256) p.bm = p.bn = 256;
+    else if (tiles(128) >= 200) p.bm = p.bn = 128;
+    const int64_t have = tiles(p.bm);
+    int64_t splits = 1;
+    if (have > 0 && have < 256) {
+        splits = (512 + have - 1) / have;
+        const int64_t most = K / (4 * bk);
+        if (splits > most) splits = most;
+        if (splits > 64) splits = 64;
+        if (splits < 1) splits = 1;
+    }
+    const int64_t per = ((K + splits - 1) / splits + bk - 1) / bk * bk;
+    p.k_split = per > 0 ? per : bk;
+    p.splits = (int)(K > 0 ? (K + p.k_split - 1) / p.k_split : 1);
+    return p;
+}
+
+static bool direct_ok(int kind, const void* p, int64_t ld, int64_t contiguous)
+{
+    // (a tile's byte offsets stay below 2^31: up to 256 rows)
+    return kind != SMLVM_F32 && aligned16(p) && ld % 8 == 0 && contiguous % 8 == 0 && ld < (1 << 20);
+}
+
+template <class T, bool ACOL, bool BCOL>
+static void launch_gemm(const Plan& p, bool direct, GemmArgs& g, hipStream_t stream)
+{
+    g.tiles_m = (int)((g.M + p.bm - 1) / p.bm);
+    g.tiles_n = (int)((g.N + p.bn - 1) / p.bn);
+    g.k_split = p.k_split;
+    const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)p.splits);
+#define GEMM(BM, BN, WM, WN, DIRECT) \
+    hipLaunchKernelGGL((gemm_kernel<T, ACOL, BCOL, BM, BN, WM, WN, DIRECT>), grid, dim3(WM * WN * 64), 0, stream, g)
+    if constexpr (sizeof(T) == 2) {
+        if (direct) {
+            if (p.bm == 256) GEMM(256, 256, 2, 4, true);
+            else if (p.bm == 128) GEMM(128, 128, 2, 2, true);
+            else GEMM(64, 64, 2, 2, true);
+            return;
+        }
+    }
+    if (p.bm == 128) GEMM(128, 128, 2, 2, false);
+    else GEMM(64, 64, 2, 2, false);
+#undef GEMM
+}
+
+template <class T>
+static void launch_join(const GemmArgs& g, int splits, hipStream_t stream)
+{
+    const int64_t blocks = (g.M * ((g.N + 3) / 4) + 255) / 256;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, g, splits);
+}
+
+// layout 0: rows x rows, 1: rows x columns, 2: columns x columns
+template <class T>
+static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
+{
+    const int kind = KindOf<T>::value;
+    const bool direct = direct_ok(kind, g.a, g.lda, layout == 2 ? g.M : g.K) && direct_ok(kind, g.b, g.ldb, layout ? g.N : g.K);
+    const Plan p = plan(kind, g.M, g.N, g.K, direct);
+    if ((double)((g.M + p.bm - 1) / p.bm) * (double)((g.N + p.bn - 1) / p.bn) > 2147483647.0) return SMLVM_ERR_UNSUPPORTED;
+    float* ws = static_cast<float*>(workspace);
+    size_t need = 0;
+    g.part = nullptr;
+    g.colsum_part = nullptr;
+    if (p.splits > 1) { g.part = ws; need += (size_t)p.splits * g.M * g.N; }
+    if (colsum) { g.colsum_part = ws + need; need += (size_t)p.splits * g.M; }
+    if (need && (!ws || bytes < need * sizeof(float))) return SMLVM_ERR_WORKSPACE;
+    if (layout == 0) launch_gemm<T, false, false>(p, direct, g, stream);
+    else if (layout == 1) launch_gemm<T, false, true>(p, direct, g, stream);
+    else launch_gemm<T, true, true>(p, direct, g, stream);
+    if (p.splits > 1) launch_join<T>(g, p.splits, stream);
+    if (colsum)
+        hipLaunchKernelGGL((join_sums_kernel<T>), dim3((unsigned)((g.M + 255) / 256)), dim3(256), 0, stream, g.colsum_part,
+                           p.splits, g.M, static_cast<T*>(colsum));
+    return check_launch();
+}
+
+static int dispatch_gemm(int kind, int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
+{
+    if (kind == SMLVM_F32) return run_gemm<float>(layout, g, colsum, workspace, bytes, stream);
+    if (kind == SMLVM_F16) return run_gemm<f16_t>(layout, g, colsum, workspace, bytes, stream);
+    return run_gemm<bf16_t>(layout, g, colsum, workspace, bytes, stream);
+}
+
+static size_t workspace_of(int kind, int64_t M, int64_t N, int64_t K, bool colsum)
+{
+    size_t most = 0;
+    for (int direct = 0; direct < 2; ++direct) {     // (which one it is depends on the pointers)
+        const Plan p = plan(kind, M, N, K, direct != 0);
+        const size_t need = (p.splits > 1 ? (size_t)p.splits * M * N : 0) + (colsum ? (size_t)p.splits * M : 0);
+        if (need > most) most = need;
+    }
+    return most * sizeof(float);
+}
+
+static bool vec4_ok(int kind, int64_t N, const void* p, int64_t ld)
+{
+    const uintptr_t mask = 4 * kind_bytes(kind) - 1;
+    return !p || (((uintptr_t)p & mask) == 0 && ld % 4 == 0 && N % 4 == 0);
+}
+
+// 0: an empty result, 1: go on, negative: an error
+static int check_sizes(int kind, int64_t M, int64_t N, int64_t K)
+{
+    if (M < 0 || N < 0 || K < 0 || !kind_ok(kind)) return SMLVM_ERR_INVALID;
+    if (M > 0x7FFFFFFF || N > 0x7FFFFFFF || K > 0x7FFFFFFF) return SMLVM_ERR_UNSUPPORTED;
+    return 1;
+}
+
+}  // namespace smlvm
+
+using namespace smlvm;
+
+extern "C" size_t smlvm_linear_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K)
+{
+    if (check_sizes(kind, M, N, K) != 1) return 0;
+    const size_t fwd = workspace_of(kind, M, N, K, false), dx = workspace_of(kind, M, K, N, false), dw = workspace_of(kind, N, K, M, true);
+    return fwd > dx ? (fwd > dw ? fwd : dw) : (dx > dw ? dx : dw);
+}
+
+extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                                const void* residual, int64_t ldr, void* y, void* pre, int32_t kind, int32_t act,
+                                int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const int go = check_sizes(kind, M, N, K);
+    if (go <= 0) return go;
+    if (act < kNone || act > kTanh) return SMLVM_ERR_INVALID;
+    if (M == 0 || N == 0) return SMLVM_OK;
+    if (!y || (K && (!x || !w)) || (K && (ldx < K || ldw < K)) || (residual && ldr < N)) return SMLVM_ERR_INVALID;
+    GemmArgs g = {};
+    g.a = x; g.b = w; g.lda = ldx; g.ldb = ldw; g.M = M; g.N = N; g.K = K;
+    g.out = y; g.bias = bias; g.res = residual; g.ldr = ldr; g.pre = pre; g.act = act;
+    g.vec = vec4_ok(kind, N, y, N) && vec4_ok(kind, N, pre, N) && vec4_ok(kind, N, residual, ldr) && vec4_ok(kind, N, bias, 0);
+    return dispatch_gemm(kind, 0, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int smlvm_linear_act_bwd(const void* dy, const void* h, void* dh, int32_t kind, int32_t act, int64_t n, void* stream_)
+{
+    if (n < 0 || !kind_ok(kind) || act < kNone || act > kTanh) return SMLVM_ERR_INVALID;
+    if (n == 0) return SMLVM_OK;
+    if (!dy || !h || !dh) return SMLVM_ERR_INVALID;
+    const hipStream_t stream = (hipStream_t)stream_;
+    const int64_t need = (n + 2047) / 2048;
+    const dim3 grid((unsigned)(need < 16384 ? need : 16384));
+    const int aligned = aligned16(dy) && aligned16(h) && aligned16(dh);
+#define ACT_BWD(T) hipLaunchKernelGGL((act_bwd_kernel<T>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
+                                      static_cast<const T*>(h), static_cast<T*>(dh), n, act, aligned)
+    if (kind == SMLVM_F32) ACT_BWD(float);
+    else if (kind == SMLVM_F16) ACT_BWD(f16_t);
+    else ACT_BWD(bf16_t);
+#undef ACT_BWD
+    return check_launch();
+}
+
+extern "C" int smlvm_linear_dx(const void* dh, int64_t ldh, const void* w, int64_t ldw, void* dx, int32_t kind, int64_t M,
+                               int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const int go = check_sizes(kind, M, N, K);
+    if (go <= 0) return go;
+    if (M == 0 || K == 0) return SMLVM_OK;
+    if (!dx || (N && (!dh || !w)) || (N && (ldh < N || ldw < K))) return SMLVM_ERR_INVALID;
+    GemmArgs g = {};
+    g.a = dh; g.b = w; g.lda = ldh; g.ldb = ldw; g.M = M; g.N = K; g.K = N;
+    g.out = dx; g.vec = vec4_ok(kind, K, dx, K);
+    return dispatch_gemm(kind, 1, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int smlvm_linear_dw(const void* dh, int64_t ldh, const void* x, int64_t ldx, void* dw, void* db, int32_t kind,
+                               int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const int go = check_sizes(kind, M, N, K);
+    if (go <= 0) return go;
+    if (N == 0 || K == 0) return SMLVM_OK;
+    if (!dw || (M && (!dh || !x)) || (M && (ldh < N || ldx < K))) return SMLVM_ERR_INVALID;
+    GemmArgs g = {};
+    g.a = dh; g.b = x; g.lda = ldh; g.ldb = ldx; g.M = N; g.N = K; g.K = M;
+    g.out = dw; g.vec = vec4_ok(kind, K, dw, K);
+    return dispatch_gemm(kind, 2, g, db, workspace, workspace_bytes, (hipStream_t)stream);
+}

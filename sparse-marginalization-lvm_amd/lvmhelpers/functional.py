@@ -260,12 +260,74 @@ def lowrank_categorical_nll(x, w, b, y):
     return _LowRankCE.apply(x.contiguous(), w.contiguous(), b.contiguous(), y)
 
 
+class _LinearAct(torch.autograd.Function):
+    """act(x w^T + b) + r with the epilogue in the product's kernel.  For the backward the forward leaves
+    act's argument (rounded to the tensors' type; relu without a residual keeps its output instead)."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, act):
+        need = any(ctx.needs_input_grad[:3])
+        own_sign = act == 1 and r is None          # relu: y > 0 exactly where its argument is
+        y, pre = _native.linear_fwd(x, w, b, r, act, want_pre=need and act != 0 and not own_sign)
+        if need:
+            ctx.act = act
+            ctx.save_for_backward(x, w, *([y if own_sign else pre] if act else []))
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = dw = db = None
+        want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
+        if want_dx or want_dw or want_db:
+            x, w = ctx.saved_tensors[:2]
+            dx, dw, db = _native.linear_bwd(dy, ctx.saved_tensors[2] if ctx.act else None, x, w, ctx.act, want_dx,
+                                            want_dw, want_db)
+        return dx, dw, db, (dy if want_dr else None), None
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """activation(x @ weight.T + bias) + residual as one kernel (split over the inner axis: two).
+
+    x [..., K], weight [N, K], bias [N], residual [..., N]: float32, float16 or bfloat16, all of one type, on one
+    GPU; residual has exactly the output's shape (nothing is broadcast).  activation: 'none', 'relu', 'gelu' (the erf
+    form), 'silu', 'sigmoid', 'tanh'.  Products are summed in fp32; float32 operands are multiplied to
+    fp32 accuracy on the bf16 matrix cores (an infinite operand may then give NaN instead of an
+    infinity).  Differentiable in all four; `bias`' gradient comes from the pass that computes `weight`'s."""
+    name = "linear_act"
+    act = _native.ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"{name}: activation must be one of {sorted(_native.ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{name}: x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
+    out_shape = x.shape[:-1] + weight.shape[:1]
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{name}: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != out_shape:
+        raise ValueError(f"{name}: residual must be {tuple(out_shape)}, got {tuple(residual.shape)}")
+    if not x.is_cuda:
+        raise _native.NativeError(f"{name}: expected GPU tensors (the hot path has no CPU fallback)")
+    if x.dtype not in _native.KINDS:
+        raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {x.dtype}")
+    for t, what in ((weight, "weight"), (bias, "bias"), (residual, "residual")):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise TypeError(f"{name}: {what} must have x's type and device ({x.dtype}, {x.device}), got {t.dtype}, {t.device}")
+    if x.dim() != 2:
+        x = x.reshape(-1, weight.shape[1]) if x.numel() else x.reshape(out_shape[:-1].numel(), weight.shape[1])
+    if residual is not None and residual.dim() != 2:
+        residual = residual.reshape(x.shape[0], weight.shape[0])
+    if bias is not None:
+        bias = bias.contiguous()
+    y = _LinearAct.apply(x, weight, bias, residual, act)
+    return y if len(out_shape) == 2 else y.view(out_shape)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """(log softmax(logits)[action], entropy) per row without the [.., V] log-probabilities."""
 
     @staticmethod
     def forward(ctx, logits, actions, mask):
         want = ctx.needs_input_grad[0]
+        ctx.set_materialize_grads(False)
         logp, entropy, stats = _native.token_logprobs_fwd(logits, actions, mask, want_stats=want)
         if want:
             ctx.has_mask = mask is not None
@@ -276,8 +338,11 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, glogp, gentropy):
         logits, actions, stats = ctx.saved_tensors[:3]
         mask = ctx.saved_tensors[3] if ctx.has_mask else None
-        return _native.token_logprobs_bwd(logits, actions, mask, stats, glogp.contiguous(),
-                                          gentropy.contiguous()), None, None
+        if glogp is None and gentropy is None:
+            return None, None, None
+        c = torch.zeros_like(gentropy) if glogp is None else glogp
+        return _native.token_logprobs_bwd(logits, actions, mask, stats, c.contiguous(),
+                                          None if gentropy is None else gentropy.contiguous()), None, None
 
 
 class _ClippedPolicyLoss(torch.autograd.Function):
@@ -292,6 +357,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coeff,
                 entropy_coeff, mean):
         want = ctx.needs_input_grad[0]
+        ctx.set_materialize_grads(False)      # (no zeros for the statistics' gradients)
         out = _native.policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff,
                                   entropy_coeff, mean, want)
         if want:
@@ -305,6 +371,8 @@ class _ClippedPolicyLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g, *_):
+        if g is None:
+            return (None,) * 11
         logits, actions, stats, c, h = ctx.saved_tensors[:5]
         mask = ctx.saved_tensors[5] if ctx.has_mask else None
         ready, ctx.ready = ctx.ready, None
@@ -320,8 +388,6 @@ def _policy_rows(logits, actions, name):
     if logits.dim() < 2 or logits.shape[-1] < 1:
         raise ValueError(f"{name}: logits must be [..., V] with at least one leading axis and V >= 1")
     lead = logits.shape[:-1]
-    if tuple(actions.shape) != tuple(lead):
-        raise ValueError(f"{name}: actions must have logits' leading shape {tuple(lead)}, got {tuple(actions.shape)}")
     if actions.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name}: actions must be int64 or int32, got {actions.dtype}")
     if logits.dim() == 2:
@@ -332,13 +398,15 @@ def _policy_rows(logits, actions, name):
 
 
 def _row_values(t, lead, logits, name, what, dtype):
-    if tuple(t.shape) != tuple(lead):
+    if t.shape != lead:
         raise ValueError(f"{name}: {what} must have logits' leading shape {tuple(lead)}, got {tuple(t.shape)}")
     if t.device != logits.device:
         raise _native.NativeError(f"{name}: {what} must be on the logits' device")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: {what} is a constant of the loss; detach it (no gradient would reach it)")
-    return t.detach().to(dtype).reshape(logits.shape[:2]).contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t.detach().reshape(logits.shape[:2]).contiguous()
 
 
 def _row_mask(mask, lead, logits, name):

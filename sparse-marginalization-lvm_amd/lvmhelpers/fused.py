@@ -26,6 +26,52 @@ from . import _native
 from . import functional as F_
 
 
+class LinearAct(torch.nn.Linear):
+    """nn.Linear with an activation and an optional residual in its epilogue (functional.linear_act); the
+    same constructor arguments, initialisation and state_dict keys as nn.Linear."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="none", **kwargs):
+        if activation not in _native.ACTIVATIONS:
+            raise ValueError(f"LinearAct: activation must be one of {sorted(_native.ACTIVATIONS)}, got {activation!r}")
+        super().__init__(in_features, out_features, bias, **kwargs)
+        self.activation = activation
+
+    def forward(self, x, residual=None):
+        return F_.linear_act(x, self.weight, self.bias, self.activation, residual)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", activation={self.activation}"
+
+
+def _activation_name(m):
+    """The epilogue that computes what module `m` does, or None."""
+    if type(m) is torch.nn.GELU:
+        return "gelu" if m.approximate == "none" else None
+    return {torch.nn.ReLU: "relu", torch.nn.SiLU: "silu", torch.nn.Sigmoid: "sigmoid", torch.nn.Tanh: "tanh"}.get(type(m))
+
+
+def fuse_linears(module):
+    """Replaces, in place, every nn.Linear inside the nn.Sequentials of `module` (itself included) by a
+    LinearAct with the same parameters, taking the activation module that follows it into the
+    epilogue; that one's place holds an nn.Identity, so that state_dict keys do not change.  Linears with
+    hooks, subclasses of nn.Linear and activations without an epilogue stay as they are.  Returns `module`."""
+    for seq in [m for m in module.modules() if isinstance(m, torch.nn.Sequential)]:
+        for i, lin in enumerate(seq):
+            if type(lin) is not torch.nn.Linear or lin._forward_hooks or lin._forward_pre_hooks:
+                continue
+            follow = seq[i + 1] if i + 1 < len(seq) else None
+            name = None if follow is None or follow._forward_hooks or follow._forward_pre_hooks else _activation_name(follow)
+            new = LinearAct.__new__(LinearAct)
+            torch.nn.Module.__init__(new)
+            new.in_features, new.out_features, new.activation = lin.in_features, lin.out_features, name or "none"
+            new.weight, new.bias = lin.weight, lin.bias        # (the same Parameters: optimisers keep them)
+            new.training = lin.training
+            seq[i] = new
+            if name is not None:
+                seq[i + 1] = torch.nn.Identity()
+    return module
+
+
 class LowRankLogits:
     """logits[n, f, c] = x[n, f, :] @ weight[c, :] + bias[c], kept factored."""
 

@@ -1,0 +1,261 @@
+"""GPU tests of linear_act (csrc/linear.hip) against the formulas in 64 bits.
+
+Tolerances, u = 2^-24.  h = x w^T + b is a sum of K products: 16-bit products are exact in fp32, each
+sum adds at most u of what is summed so far (any order: (K + splits) u sum |x||w|, far from reached; the
+bound below uses min(K, 64) + 8 + K / 64 for sums that run 32 k at a time per instruction);
+float32 adds 2^-22 sum |x||w| for the parts left out and the six products' own sums.  An activation's
+slope is at most 1.13, its own error 4 u |.| + 4 u.  Results are rounded by half a step of the type;
+the backward starts from h (dh) rounded once to the type: half a step of it, relative, into
+every product with it, and half a step of h times |act''| <= 1 into dh."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+ACTS = ["none", "relu", "gelu", "silu", "sigmoid", "tanh"]
+
+
+def _F():
+    from lvmhelpers import functional
+    return functional
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _sum_err(K, dtype):
+    return U * (min(K, 64) + 8 + K / 64 + (4 + 6 * (min(K, 64) + 8 + K / 64) / 16 if dtype == torch.float32 else 0))
+
+
+def _act(name, h):
+    return {"none": lambda: h, "relu": lambda: h.clamp_min(0), "gelu": lambda: torch.nn.functional.gelu(h),
+            "silu": lambda: torch.nn.functional.silu(h), "sigmoid": lambda: torch.sigmoid(h),
+            "tanh": lambda: torch.tanh(h)}[name]()
+
+
+def _case(M, N, K, dtype, seed, bias=True, res=False):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    return ((r(M, K)).to(dtype), (r(N, K) * max(K, 1) ** -0.5).to(dtype), (r(N) * 0.5).to(dtype) if bias else None,
+            r(M, N).to(dtype) if res else None, r(M, N).to(dtype))
+
+
+def _within(got, want, tol):
+    assert got.shape == want.shape
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), (float((off - tol).max()), float(off.max()))
+
+
+def _check(dev, x, w, b, r, dy, act, dtype, run=None, grads=True):
+    M, K = x.shape
+    N = w.shape[0]
+    leaves = [None if t is None else t.to(dev).requires_grad_(grads) for t in (x, w, b, r)]
+    y = (run or _F().linear_act)(leaves[0], leaves[1], leaves[2], act, leaves[3])
+    # the reference, on the GPU in fp64 where it is large
+    where = dev if M * N * K > 1 << 24 else "cpu"
+    X, W, B, R, DY = (None if t is None else t.to(where).double() for t in (x, w, b, r, dy))
+    h = X @ W.t().contiguous()
+    mag = X.abs() @ W.abs().t().contiguous()
+    if B is not None:
+        h, mag = h + B, mag + B.abs()
+    h = h.requires_grad_(True)
+    a = _act(act, h)
+    want = a + (R if R is not None else 0)
+    half = _half(dtype) if dtype != torch.float32 else U
+    herr = _sum_err(K, dtype) * mag
+    aerr = 1.13 * herr + 8 * U * (a.detach().abs() + 1 * (act not in ("none", "relu")))
+    _within(y.detach(), want.detach().cpu(), (aerr + half * want.detach().abs() * 1.01 + 2 * U * (R.abs() if R is not None else 0) + 2.0 ** -25 * (dtype == torch.float16)).cpu())
+    if not grads:
+        return
+    (dh,) = torch.autograd.grad(a, h, DY)
+    hd = h.detach()
+    near = (hd.abs() <= herr).double() if act == "relu" else 0.0        # relu's corner may fall either way
+    # dh: slope at the rounded h, then rounded
+    dherr = DY.abs() * (1.01 * (herr + half * hd.abs() * (dtype != torch.float32)) * (act not in ("none", "relu")) + 12 * U + near) + half * dh.abs() * (
+        dtype != torch.float32 and act != "none") + 2.0 ** -25 * (dtype == torch.float16)
+    got = torch.autograd.grad(y, [t for t in leaves if t is not None], dy.to(dev))
+    got = iter(got)
+    Wc, Xc = W.contiguous(), X
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -120
+    want_dx = dh @ Wc
+    _within(next(got), want_dx.cpu(), (dherr @ Wc.abs() + _sum_err(N, dtype) * (dh.abs() @ Wc.abs()) + half * want_dx.abs() * 1.01 + tiny).cpu())
+    dht = dh.t().contiguous()
+    want_dw = dht @ Xc
+    _within(next(got), want_dw.cpu(), (dherr.t().contiguous() @ Xc.abs() + _sum_err(M, dtype) * (dht.abs() @ Xc.abs()) + half * want_dw.abs() * 1.01 + tiny).cpu())
+    if b is not None:
+        want_db = dh.sum(0)
+        _within(next(got), want_db.cpu(), (dherr.sum(0) + _sum_err(M, dtype) * dh.abs().sum(0) + half * want_db.abs() * 1.01 + tiny).cpu())
+    if r is not None:
+        assert torch.equal(next(got).cpu(), dy)
+
+
+# below, at and over every tile and fragment edge; odd widths take the unaligned path
+SIZES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (1, 64, 64), (17, 16, 32), (64, 64, 64), (65, 63, 66), (128, 128, 128),
+         (127, 129, 257), (200, 72, 1000), (1, 4096, 512), (3, 1000, 777), (5000, 8, 16), (4097, 24, 40), (300, 784, 16),
+         (33, 1024, 8), (256, 256, 72)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_every_size(dev, M, N, K, dtype):
+    _check(dev, *_case(M, N, K, dtype, M + N + K), "gelu", dtype)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias,res", [(True, True), (False, False), (False, True)])
+def test_every_epilogue(dev, act, bias, res, dtype):
+    for M, N, K in ((70, 96, 48), (70, 97, 47)):
+        _check(dev, *_case(M, N, K, dtype, 5, bias, res), act, dtype)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4160, 4352, 200), (2048, 2048, 1024), (1, 64, 70000), (20000, 16, 24)])
+def test_large_tiles_and_long_sums(dev, M, N, K, dtype):
+    """The 256 x 256 and 128 x 128 tiles (full and partly filled), and products split over a long axis."""
+    _check(dev, *_case(M, N, K, dtype, 1), "silu", dtype)
+
+
+def test_fp32_keeps_fp32_accuracy(dev):
+    """Values over 60 binades and sums that cancel: three bf16 parts carry all 24 bits."""
+    g = torch.Generator().manual_seed(0)
+    M, N, K = 64, 64, 256
+    x = torch.randn(M, K, generator=g) * torch.exp2(torch.randint(-30, 31, (M, 1), generator=g).float())
+    w = torch.randn(N, K, generator=g) * torch.exp2(torch.randint(-30, 31, (N, 1), generator=g).float())
+    x[:, 128:] = -x[:, :128] * (1 + 2.0 ** -20)
+    w[:, 128:] = w[:, :128]
+    y = _F().linear_act(x.to(dev), w.to(dev))
+    want = x.double() @ w.double().t()
+    _within(y, want, _sum_err(K, torch.float32) * (x.double().abs() @ w.double().abs().t()))
+    one = torch.eye(64) * 1.2345678           # a single product per sum
+    w = w[:, :64].contiguous()
+    _within(F_one(one.to(dev), w.to(dev)), one.double() @ w.double().t(), 4 * U * (one.double() @ w.double().abs().t()))
+
+
+def F_one(x, w):
+    return _F().linear_act(x, w)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_strided_operands(dev, dtype):
+    """Rows a distance apart, a transposed weight, x and residual with more axes."""
+    F_ = _F()
+    x, w, b, r, dy = _case(24, 40, 32, dtype, 3, True, True)
+    base = F_.linear_act(*(t.to(dev) for t in (x, w, b)), "tanh", r.to(dev))
+    wide = torch.zeros(24, 50, dtype=dtype)
+    wide[:, 9:41] = x
+    rw = torch.zeros(24, 64, dtype=dtype)
+    rw[:, 8:48] = r
+    assert torch.equal(F_.linear_act(wide.to(dev)[:, 9:41], w.to(dev), b.to(dev), "tanh", rw.to(dev)[:, 8:48]), base)
+    assert torch.equal(F_.linear_act(x.to(dev), w.t().contiguous().to(dev).t(), b.to(dev), "tanh", r.to(dev)), base)
+    assert torch.equal(F_.linear_act(x.view(2, 3, 4, 32).to(dev), w.to(dev), b.to(dev), "tanh", r.view(2, 3, 4, 40).to(dev)),
+                       base.view(2, 3, 4, 40))
+    xt = x.t().contiguous().to(dev).t()                       # column-major x
+    assert torch.equal(F_.linear_act(xt, w.to(dev), b.to(dev), "tanh", r.to(dev)), base)
+    one = F_.linear_act(x[0].to(dev), w.to(dev), b.to(dev), "tanh", r[0].to(dev))
+    assert one.shape == (40,)
+    _within(one, base[0].double().cpu(), 4 * _half(dtype) * base[0].double().cpu().abs() + 1e-6)
+    # gradients through views, an expanded dy, and a frozen weight
+    big = wide.to(dev).requires_grad_(True)
+    F_.linear_act(big[:, 9:41], w.to(dev), b.to(dev), "tanh").sum().backward()
+    assert bool((big.grad[:, :9] == 0).all()) and bool((big.grad[:, 41:] == 0).all()) and float(big.grad.abs().sum()) > 0
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_empty_axes(dev, dtype):
+    F_ = _F()
+    b = torch.arange(5, dtype=dtype, device=dev).requires_grad_(True)
+    y = F_.linear_act(torch.empty(3, 0, dtype=dtype, device=dev), torch.empty(5, 0, dtype=dtype, device=dev), b, "relu")
+    assert torch.equal(y, b.detach().expand(3, 5))
+    y.sum().backward()
+    assert torch.equal(b.grad.cpu(), torch.tensor([0, 3, 3, 3, 3], dtype=dtype))
+    x = torch.empty(0, 4, dtype=dtype, device=dev, requires_grad=True)
+    w = torch.ones(5, 4, dtype=dtype, device=dev, requires_grad=True)
+    b.grad = None
+    y = F_.linear_act(x, w, b, "gelu")
+    y.sum().backward()
+    assert y.shape == (0, 5) and x.grad.shape == (0, 4) and bool((w.grad == 0).all()) and bool((b.grad == 0).all())
+    assert F_.linear_act(torch.ones(2, 4, dtype=dtype, device=dev), w.detach()[:0]).shape == (2, 0)
+
+
+def test_nan_stays_in_its_rows(dev):
+    for dtype in FLOATS:
+        x, w, b, _, _ = _case(40, 72, 64, dtype, 3)
+        clean = _F().linear_act(x.to(dev), w.to(dev), b.to(dev), "relu")
+        x[7, 3] = float("nan")
+        x[9, 0] = float("inf")
+        y = _F().linear_act(x.to(dev), w.to(dev), b.to(dev), "relu")
+        keep = [i for i in range(40) if i not in (7, 9)]
+        assert torch.equal(y[keep], clean[keep]) and bool(y[7].isnan().all())
+
+
+def test_neighbouring_memory_is_left_alone(dev):
+    """Rows behind the last one, and what lies between the rows of strided inputs (NaN there)."""
+    for dtype in FLOATS:
+        for M, N, K in ((5, 72, 64), (5, 70, 61)):
+            x, w, b, _, _ = _case(M, N, K, dtype, 3)
+            xb = torch.full((M + 4, K + 8), float("nan"), dtype=dtype, device=dev)
+            xb[:M, :K] = x.to(dev)
+            wb = torch.full((N + 4, K + 8), float("nan"), dtype=dtype, device=dev)
+            wb[:N, :K] = w.to(dev)
+            y = _F().linear_act(xb[:M, :K], wb[:N, :K], b.to(dev), "gelu")
+            assert bool(y.isfinite().all())
+            base = _F().linear_act(x.to(dev), w.to(dev), b.to(dev), "gelu")
+            _within(y, base.double().cpu(), 4 * _half(dtype) * base.double().cpu().abs() + 1e-5)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_captured_streams_and_repeats(dev, dtype):
+    from lvmhelpers import graphs
+    F_ = _F()
+    x, w, b, r, dy = (t.to(dev) for t in _case(300, 200, 1200, dtype, 3, True, True))
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    held = {}
+
+    def step():
+        y = F_.linear_act(x, w, b, "gelu", r)
+        held["out"] = [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, _ = graphs.capture(step)
+    out = held["out"]
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(300, 1200, generator=torch.Generator().manual_seed(k)).to(dtype))
+        graph.replay()
+        torch.randn(99, device=dev).sum().item()
+        step()
+        assert all(torch.equal(p, q) for p, q in zip(out, held["out"]))
+
+
+def test_modules_are_drop_ins(dev):
+    """fuse_linears keeps parameters and state_dict keys, takes activations in, and leaves what it cannot."""
+    from lvmhelpers import fused
+    torch.manual_seed(0)
+    def make():
+        return torch.nn.Sequential(torch.nn.Linear(20, 48), torch.nn.ReLU(), torch.nn.Linear(48, 30), torch.nn.GELU(approximate="tanh"),
+                                   torch.nn.Sequential(torch.nn.Linear(30, 7, bias=False), torch.nn.Sigmoid()))
+    plain = make()
+    net = make()
+    net.load_state_dict(plain.state_dict())
+    params = list(net.parameters())
+    assert fused.fuse_linears(net) is net
+    assert [n for n, _ in net.named_parameters()] == [n for n, _ in plain.named_parameters()]
+    assert all(p is q for p, q in zip(params, net.parameters()))
+    assert net[0].activation == "relu" and net[2].activation == "none" and isinstance(net[3], torch.nn.GELU)
+    assert net[4][0].activation == "sigmoid" and net[4][0].bias is None and "sigmoid" in repr(net)
+    plain, net = plain.to(dev).double(), net.to(dev)
+    x = torch.randn(9, 20)
+    want = plain(x.to(dev).double())
+    got = net(x.to(dev))
+    assert float((got.double() - want).abs().max()) <= 200 * U
+    want.sum().backward()
+    got.sum().backward()
+    for p, q in zip(plain.parameters(), net.parameters()):
+        assert float((p.grad - q.grad.double()).abs().max()) <= 2000 * U * (1 + float(p.grad.abs().max()))

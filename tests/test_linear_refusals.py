@@ -1,0 +1,64 @@
+"""CPU: what linear_act, its module and its C entries refuse."""
+import ctypes
+
+import pytest
+import torch
+
+from lvmhelpers import _native, fused
+from lvmhelpers import functional as F_
+
+
+@pytest.mark.parametrize("args,error", [
+    ((torch.zeros(2, 3), torch.zeros(4, 3)), _native.NativeError),
+    ((torch.zeros(2, 3), torch.zeros(4, 5)), ValueError),
+    ((torch.zeros(2, 3), torch.zeros(3)), ValueError),
+    ((torch.zeros(2, 3), torch.zeros(4, 3), torch.zeros(3)), ValueError),
+    ((torch.zeros(2, 3), torch.zeros(4, 3), None, "softplus"), ValueError),
+    ((torch.zeros(2, 3), torch.zeros(4, 3), None, "none", torch.zeros(4)), ValueError),       # no broadcasting
+    ((torch.zeros(2, 3), torch.zeros(4, 3), None, "none", torch.zeros(1, 4)), ValueError),
+])
+def test_refusals(args, error):
+    with pytest.raises(error):
+        F_.linear_act(*args)
+
+
+def test_module_refuses_unknown_activations():
+    with pytest.raises(ValueError):
+        fused.LinearAct(3, 4, activation="softplus")
+    assert list(fused.LinearAct(3, 4, activation="relu").state_dict()) == ["weight", "bias"]
+
+
+def test_fuse_linears_leaves_hooks_and_subclasses():
+    class Mine(torch.nn.Linear):
+        pass
+    hooked = torch.nn.Linear(3, 3)
+    hooked.register_forward_hook(lambda *a: None)
+    act = torch.nn.ReLU()
+    act.register_forward_hook(lambda *a: None)
+    net = fused.fuse_linears(torch.nn.Sequential(Mine(3, 3), hooked, torch.nn.Linear(3, 3), act, torch.nn.Linear(3, 2)))
+    assert type(net[0]) is Mine and net[1] is hooked and net[2].activation == "none" and net[3] is act
+    assert type(net[4]) is fused.LinearAct
+
+
+def test_c_entries_check_their_arguments():
+    L = _native.lib()
+    i64, i32, sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
+    one = ctypes.c_void_p(16)
+    big = L.smlvm_linear_workspace_bytes(0, 4, 64, 100000)
+    assert big > 0 and L.smlvm_linear_workspace_bytes(0, 4, 4, 4) >= 16      # (column sums)
+    assert L.smlvm_linear_workspace_bytes(7, 4, 4, 4) == 0
+    for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0), (0, 0, 0)):                # empty axes
+        assert L.smlvm_linear_workspace_bytes(0, *sizes) >= 0 and L.smlvm_linear_workspace_bytes(2, *sizes) >= 0
+
+    def fwd(x=one, ldx=100000, w=one, y=one, kind=0, act=0, M=4, N=64, K=100000, ws=one, nbytes=big, r=None, ldr=64):
+        return L.smlvm_linear_fwd(x, i64(ldx), w, i64(max(K, 1)), None, r, i64(ldr), y, None, i32(kind), i32(act), i64(M), i64(N),
+                                  i64(K), ws, sz(nbytes), None)
+    assert fwd(M=0) == 0 and fwd(N=0) == 0
+    assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1 and fwd(kind=3) == -1 and fwd(act=6) == -1
+    assert fwd(ldx=99999) == -1 and fwd(r=one, ldr=63) == -1 and fwd(M=-1) == -1 and fwd(M=1 << 31) == -2
+    assert fwd(ws=None, nbytes=0) == -4 and fwd(nbytes=1) == -4                    # the split product's partial sums
+    assert L.smlvm_linear_act_bwd(one, None, one, i32(0), i32(1), i64(4), None) == -1
+    assert L.smlvm_linear_act_bwd(None, None, None, i32(0), i32(1), i64(0), None) == 0
+    assert L.smlvm_linear_dx(None, i64(4), one, i64(4), one, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -1
+    assert L.smlvm_linear_dw(one, i64(4), one, i64(4), one, one, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -4
+    assert L.smlvm_linear_dw(one, i64(4), one, i64(4), None, None, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -1
