@@ -33,26 +33,62 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5 };
 
-__device__ __forceinline__ float sigmoid_f(float h) { return 1.0f / (1.0f + expf(-h)); }
+// FAST (16-bit results): reciprocals and exponentials of the hardware's precision, and Phi(h) from a fit of
+// log(erfc(z) e^(z^2) / t) by a polynomial in t = 1 / (1 + 0.3 z) on 0 <= z <= 9.5 (least squares, reweighted to an
+// even error of 4.3e-7): gelu is off by 2e-7 at most, a hundredth of half a step of fp16 near 0.01, and
+// costs 14 instructions where erff, both of whose branches a wave takes, costs 50 (the 8192 x 8192 forward
+// with it spent 300 us of 820 in the epilogue).
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_f(float h)
+{
+    if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * h));
+    else return 1.0f / (1.0f + expf(-h));
+}
+// the normal distribution function
+template <bool FAST>
+__device__ __forceinline__ float phi_f(float h)
+{
+    if constexpr (FAST) {
+        const float z = fabsf(h) * 0.70710678f;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, z, 1.0f));
+        float p = 0.485700458f;
+        p = fmaf(p, t, -1.98586082f);
+        p = fmaf(p, t, 2.91078472f);
+        p = fmaf(p, t, -2.12544775f);
+        p = fmaf(p, t, 1.27865398f);
+        p = fmaf(p, t, 0.173279762f);
+        p = fmaf(p, t, 1.04183877f);
+        p = fmaf(p, t, -1.77894974f);
+        const float half = 0.5f * t * __builtin_amdgcn_exp2f(fmaf(-z, z, p) * 1.44269504f);
+        return h >= 0.0f ? 1.0f - half : half;
+    } else {
+        return 0.5f * (1.0f + erff(h * 0.70710678118654752f));
+    }
+}
 
+template <bool FAST>
 __device__ __forceinline__ float act_f(int act, float h)
 {
     switch (act) {
         case kRelu: return h > 0.0f ? h : (h != h ? h : 0.0f);
-        case kGelu: return 0.5f * h * (1.0f + erff(h * 0.70710678118654752f));
-        case kSilu: return h * sigmoid_f(h);
-        case kSigmoid: return sigmoid_f(h);
+        case kGelu: return h * phi_f<FAST>(h);
+        case kSilu: return h * sigmoid_f<FAST>(h);
+        case kSigmoid: return sigmoid_f<FAST>(h);
         case kTanh: return tanhf(h);
         default: return h;
     }
 }
+template <bool FAST>
 __device__ __forceinline__ float act_slope_f(int act, float h)
 {
     switch (act) {
         case kRelu: return h > 0.0f ? 1.0f : 0.0f;
-        case kGelu: return 0.5f * (1.0f + erff(h * 0.70710678118654752f)) + h * 0.39894228040143268f * expf(-0.5f * h * h);
-        case kSilu: { const float s = sigmoid_f(h); return s * (1.0f + h * (1.0f - s)); }
-        case kSigmoid: { const float s = sigmoid_f(h); return s * (1.0f - s); }
+        case kGelu: {
+            const float e = FAST ? __builtin_amdgcn_exp2f(-0.72134752f * h * h) : expf(-0.5f * h * h);
+            return fmaf(h * 0.39894228040143268f, e, phi_f<FAST>(h));
+        }
+        case kSilu: { const float s = sigmoid_f<FAST>(h); return s * (1.0f + h * (1.0f - s)); }
+        case kSigmoid: { const float s = sigmoid_f<FAST>(h); return s * (1.0f - s); }
         case kTanh: { const float t = tanhf(h); return 1.0f - t * t; }
         default: return 1.0f;
     }
@@ -68,7 +104,8 @@ struct GemmArgs {
     int64_t ldr;
     void* pre;                    // nullable: act's argument [M][N]
     float* part;                  // not null: fp32 partial sums [splits][M][N] instead of out
-    float* colsum_part;           // not null (column a): fp32 sums over k of A(m, k), [splits][M]
+    float* colsum_part;           // not null (column a, split): fp32 sums over k of A(m, k), [splits][M]
+    void* colsum;                 // not null (column a): sums over k of A(m, k), [M]
     int act;
     int vec;                      // out, pre, res and bias may be accessed 4 elements at a time
     int tiles_m, tiles_n;
@@ -97,6 +134,21 @@ __device__ __forceinline__ void store4(T* p, bool vec, int have, const float (&x
     }
 }
 
+// act's argument for the backward: fp32, or fp16 next to 16-bit tensors of either type.  fp16 keeps 11 bits where
+// bf16 keeps 8, so that the slope taken from it adds nothing to the rounding of dh itself (with bf16 the
+// gradients were 1.6 times as far from exact ones as their own type's rounding, so 1.4); beyond its
+// range every activation's slope is constant.
+template <class T> struct PreOf { typedef f16_t type; };
+template <> struct PreOf<float> { typedef float type; };
+template <class T>
+__device__ __forceinline__ void store_pre(void* pre, int64_t at, bool vec, int have, const float (&x)[4])
+{
+    float h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = sizeof(T) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    store4(static_cast<typename PreOf<T>::type*>(pre) + at, vec, have, h);
+}
+
 // 4 consecutive n of row m: bias, activation, residual, stores
 template <class T>
 __device__ __forceinline__ void finish4(const GemmArgs& g, int64_t m, int64_t n, float (&x)[4])
@@ -109,10 +161,10 @@ __device__ __forceinline__ void finish4(const GemmArgs& g, int64_t m, int64_t n,
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] += b[j];
     }
-    if (g.pre) store4(static_cast<T*>(g.pre) + m * g.N + n, vec, have, x);
+    if (g.pre) store_pre<T>(g.pre, m * g.N + n, vec, have, x);
     if (g.act != kNone) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = act_f(g.act, x[j]);
+        for (int j = 0; j < 4; ++j) x[j] = act_f<sizeof(T) == 2>(g.act, x[j]);
     }
     if (g.res) {
         float r[4];
@@ -309,9 +361,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
     using TA = Tile<BM, BK, ACOL>;
     using TB = Tile<BN, BK, BCOL>;
     constexpr int STAGE = PLANES * (TA::kBytes + TB::kBytes);
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+    // Through registers one buffer does: the next tile waits in registers, and two or three workgroups per
+    // CU fill each other's gaps (two buffers of the fp32 planes would leave room for one).
+    __shared__ __attribute__((aligned(16))) char lds[(DIRECT ? 2 : 1) * STAGE];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // (wave in a scalar register: matrix instructions ignore the exec mask, so what skips one has to be a
+    // scalar branch)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the 8 XCDs: give each XCD, with its own L2, one stretch of tiles, walked in
     // groups of 8 row tiles so that its neighbours share operands.
     int id = blockIdx.x;
@@ -328,16 +384,17 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
     const int64_t k_begin = (int64_t)blockIdx.z * g.k_split;
     const int64_t k_end = g.K < k_begin + g.k_split ? g.K : k_begin + g.k_split;
     const int mw = (wave / WN) * (BM / WM), nw = (wave % WN) * (BN / WN);
-    const bool colsum = ACOL && g.colsum_part && n0 == 0 && wave % WN == 0;
+    const bool colsum = ACOL && g.colsum && n0 == 0;
+    constexpr int FS = ACOL ? FM / WN : 1;                              // a wave's share of its rows' column sums
 
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    f32x4 sums[ACOL ? FM : 1];
+    f32x4 sums[FS];
 #pragma unroll
-    for (int i = 0; i < (ACOL ? FM : 1); ++i) sums[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < FS; ++i) sums[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr short kOne = KindOf<T>::value == SMLVM_F16 ? 0x3C00 : 0x3F80;
     const s16x8 ones = {kOne, kOne, kOne, kOne, kOne, kOne, kOne, kOne};
 
@@ -346,6 +403,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
         const char* const tb = stage + PLANES * TA::kBytes;
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
+            if constexpr (FM * FN >= 32) __builtin_amdgcn_sched_barrier(0);   // (one step's operands at a time: registers)
             s16x8 af[PLANES][FM], bf[PLANES][FN];
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
@@ -370,9 +428,11 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
             if constexpr (ACOL) {
                 if (colsum) {
 #pragma unroll
-                    for (int i = 0; i < FM; ++i)
+                    for (int i = 0; i < FM; ++i) {
+                        if (i / FS != wave % WN) continue;               // (uniform)
 #pragma unroll
-                        for (int q = PLANES - 1; q >= 0; --q) sums[i] = mfma<T>(ones, af[q][i], sums[i]);
+                        for (int q = PLANES - 1; q >= 0; --q) sums[i % FS] = mfma<T>(ones, af[q][i], sums[i % FS]);
+                    }
                 }
             }
         }
@@ -409,21 +469,17 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
         if (steps > 0) {
             sa.load(a, g.lda, m0, g.M, k_begin, k_end);
             sb.load(b, g.ldb, n0, g.N, k_begin, k_end);
-            sa.store(lds);
-            sb.store(lds + PLANES * TA::kBytes);
         }
         for (int64_t s = 0; s < steps; ++s) {
+            __syncthreads();                                             // (the last tile has been read)
+            sa.store(lds);
+            sb.store(lds + PLANES * TA::kBytes);
             __syncthreads();
             if (s + 1 < steps) {
                 sa.load(a, g.lda, m0, g.M, k_begin + (s + 1) * BK, k_end);
                 sb.load(b, g.ldb, n0, g.N, k_begin + (s + 1) * BK, k_end);
             }
-            compute(lds + (s & 1) * STAGE);
-            if (s + 1 < steps) {
-                char* const to = lds + ((s + 1) & 1) * STAGE;
-                sa.store(to);
-                sb.store(to + PLANES * TA::kBytes);
-            }
+            compute(lds);
         }
     }
 
@@ -445,17 +501,29 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
             }
         }
         if constexpr (ACOL) {
-            if (colsum && lane < 16) g.colsum_part[(int64_t)blockIdx.z * g.M + m] = sums[i].x;
+            if (colsum && lane < 16 && i / FS == wave % WN) {
+                if (g.colsum_part) g.colsum_part[(int64_t)blockIdx.z * g.M + m] = sums[i % FS].x;
+                else static_cast<T*>(g.colsum)[m] = (T)sums[i % FS].x;
+            }
         }
     }
 }
 
-// Joins the partial sums of a split product, in order, and runs the epilogue.
+// Joins the partial sums of a split product, in order, and runs the epilogue; the workgroups behind the
+// first `blocks` join the column sums.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits)
+__global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits, int blocks)
 {
+    if ((int)blockIdx.x >= blocks) {
+        const int64_t m = (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x;
+        if (m >= g.M) return;
+        float s = 0.0f;
+        for (int z = 0; z < splits; ++z) s += g.colsum_part[(int64_t)z * g.M + m];
+        static_cast<T*>(g.colsum)[m] = (T)s;
+        return;
+    }
     const int64_t per_row = (g.N + 3) / 4, total = g.M * per_row;
-    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
         const int64_t m = v / per_row, n = (v - m * per_row) * 4;
         const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -469,33 +537,22 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits)
     }
 }
 
-// Column sums: db[m] = sum over the splits.
-template <class T>
-__global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict__ part, int splits, int64_t M, T* __restrict__ out)
-{
-    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (m >= M) return;
-    float s = 0.0f;
-    for (int z = 0; z < splits; ++z) s += part[(int64_t)z * M + m];
-    out[m] = (T)s;
-}
-
-// dh = dy act'(h); relu may be given y in the place of h (the sign is the same).
-template <class T>
-__global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ h, T* __restrict__ dh,
+// dh = dy act'(h), H the type h is kept in; relu may be given y in the place of h (the sign is the same).
+template <class T, class H>
+__global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, const H* __restrict__ h, T* __restrict__ dh,
                                                       int64_t n, int act, int aligned)
 {
     const int64_t stride = (int64_t)gridDim.x * 256 * 8;
     for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < n; at += stride) {
         float x[8], y[8];
         if (aligned && at + 8 <= n) {
-            load_vec<T, 8>(h + at, x);
+            load_vec<H, 8>(h + at, x);
             load_vec<T, 8>(dy + at, y);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= act_slope_f(act, x[j]);
+            for (int j = 0; j < 8; ++j) y[j] *= act_slope_f<sizeof(T) == 2>(act, x[j]);
             store_vec<T, 8>(dh + at, y);
         } else {
-            for (int j = 0; j < 8 && at + j < n; ++j) dh[at + j] = (T)((float)dy[at + j] * act_slope_f(act, (float)h[at + j]));
+            for (int j = 0; j < 8 && at + j < n; ++j) dh[at + j] = (T)((float)dy[at + j] * act_slope_f<sizeof(T) == 2>(act, (float)h[at + j]));
         }
     }
 }
@@ -538,6 +595,7 @@ static void launch_gemm(const Plan& p, bool direct, GemmArgs& g, hipStream_t str
 {
     g.tiles_m = (int)((g.M + p.bm - 1) / p.bm);
     g.tiles_n = (int)((g.N + p.bn - 1) / p.bn);
+    if (g.tiles_n == 0) g.tiles_n = 1;               // (column sums alone)
     g.k_split = p.k_split;
     const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)p.splits);
 #define GEMM(BM, BN, WM, WN, DIRECT) \
@@ -555,13 +613,6 @@ static void launch_gemm(const Plan& p, bool direct, GemmArgs& g, hipStream_t str
 #undef GEMM
 }
 
-template <class T>
-static void launch_join(const GemmArgs& g, int splits, hipStream_t stream)
-{
-    const int64_t blocks = (g.M * ((g.N + 3) / 4) + 255) / 256;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, g, splits);
-}
-
 // layout 0: rows x rows, 1: rows x columns, 2: columns x columns
 template <class T>
 static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
@@ -572,18 +623,25 @@ static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size
     if ((double)((g.M + p.bm - 1) / p.bm) * (double)((g.N + p.bn - 1) / p.bn) > 2147483647.0) return SMLVM_ERR_UNSUPPORTED;
     float* ws = static_cast<float*>(workspace);
     size_t need = 0;
-    g.part = nullptr;
-    g.colsum_part = nullptr;
-    if (p.splits > 1) { g.part = ws; need += (size_t)p.splits * g.M * g.N; }
-    if (colsum) { g.colsum_part = ws + need; need += (size_t)p.splits * g.M; }
+    g.colsum = colsum;
+    if (p.splits > 1) {
+        g.part = ws;
+        need += (size_t)p.splits * g.M * g.N;
+        if (colsum) {
+            g.colsum_part = ws + need;
+            need += (size_t)p.splits * g.M;
+        }
+    }
     if (need && (!ws || bytes < need * sizeof(float))) return SMLVM_ERR_WORKSPACE;
     if (layout == 0) launch_gemm<T, false, false>(p, direct, g, stream);
     else if (layout == 1) launch_gemm<T, false, true>(p, direct, g, stream);
     else launch_gemm<T, true, true>(p, direct, g, stream);
-    if (p.splits > 1) launch_join<T>(g, p.splits, stream);
-    if (colsum)
-        hipLaunchKernelGGL((join_sums_kernel<T>), dim3((unsigned)((g.M + 255) / 256)), dim3(256), 0, stream, g.colsum_part,
-                           p.splits, g.M, static_cast<T*>(colsum));
+    if (p.splits > 1) {
+        const int64_t want = (g.M * ((g.N + 3) / 4) + 255) / 256;
+        const int blocks = (int)(want < 8192 ? want : 8192);
+        const int64_t sums = colsum ? (g.M + 255) / 256 : 0;
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + sums)), dim3(256), 0, stream, g, p.splits, blocks);
+    }
     return check_launch();
 }
 
@@ -599,7 +657,7 @@ static size_t workspace_of(int kind, int64_t M, int64_t N, int64_t K, bool colsu
     size_t most = 0;
     for (int direct = 0; direct < 2; ++direct) {     // (which one it is depends on the pointers)
         const Plan p = plan(kind, M, N, K, direct != 0);
-        const size_t need = (p.splits > 1 ? (size_t)p.splits * M * N : 0) + (colsum ? (size_t)p.splits * M : 0);
+        const size_t need = p.splits > 1 ? (size_t)p.splits * M * (N + (colsum ? 1 : 0)) : 0;
         if (need > most) most = need;
     }
     return most * sizeof(float);
@@ -611,7 +669,10 @@ static bool vec4_ok(int kind, int64_t N, const void* p, int64_t ld)
     return !p || (((uintptr_t)p & mask) == 0 && ld % 4 == 0 && N % 4 == 0);
 }
 
-// 0: an empty result, 1: go on, negative: an error
+// dh, in front of the products' partial sums
+static size_t act_bytes(int kind, int64_t M, int64_t N) { return ((size_t)M * N * kind_bytes(kind) + 15) & ~(size_t)15; }
+
+// 1: go on, negative: an error
 static int check_sizes(int kind, int64_t M, int64_t N, int64_t K)
 {
     if (M < 0 || N < 0 || K < 0 || !kind_ok(kind)) return SMLVM_ERR_INVALID;
@@ -623,11 +684,16 @@ static int check_sizes(int kind, int64_t M, int64_t N, int64_t K)
 
 using namespace smlvm;
 
-extern "C" size_t smlvm_linear_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K)
+extern "C" size_t smlvm_linear_fwd_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K)
+{
+    return check_sizes(kind, M, N, K) == 1 ? workspace_of(kind, M, N, K, false) : 0;
+}
+
+extern "C" size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, int64_t M, int64_t N, int64_t K)
 {
     if (check_sizes(kind, M, N, K) != 1) return 0;
-    const size_t fwd = workspace_of(kind, M, N, K, false), dx = workspace_of(kind, M, K, N, false), dw = workspace_of(kind, N, K, M, true);
-    return fwd > dx ? (fwd > dw ? fwd : dw) : (dx > dw ? dx : dw);
+    const size_t dx = workspace_of(kind, M, K, N, false), dw = workspace_of(kind, N, K, M, true);
+    return (dx > dw ? dx : dw) + (act ? act_bytes(kind, M, N) : 0);
 }
 
 extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -635,7 +701,7 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
                                 int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
 {
     const int go = check_sizes(kind, M, N, K);
-    if (go <= 0) return go;
+    if (go < 0) return go;
     if (act < kNone || act > kTanh) return SMLVM_ERR_INVALID;
     if (M == 0 || N == 0) return SMLVM_OK;
     if (!y || (K && (!x || !w)) || (K && (ldx < K || ldw < K)) || (residual && ldr < N)) return SMLVM_ERR_INVALID;
@@ -646,46 +712,49 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
     return dispatch_gemm(kind, 0, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int smlvm_linear_act_bwd(const void* dy, const void* h, void* dh, int32_t kind, int32_t act, int64_t n, void* stream_)
+extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int32_t h_is_y, const void* x, int64_t ldx,
+                                const void* w, int64_t ldw, void* dx, void* dw, void* db, int32_t kind, int32_t act,
+                                int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream_)
 {
-    if (n < 0 || !kind_ok(kind) || act < kNone || act > kTanh) return SMLVM_ERR_INVALID;
-    if (n == 0) return SMLVM_OK;
-    if (!dy || !h || !dh) return SMLVM_ERR_INVALID;
+    const int go = check_sizes(kind, M, N, K);
+    if (go < 0) return go;
+    if (act < kNone || act > kTanh || (h_is_y && act != kRelu) || (db && !dw && K)) return SMLVM_ERR_INVALID;
+    const bool some = M && N;                                            // dy is not empty
+    if ((some && (!dy || ldy < N || (act && (!h || ldy != N)))) || (dx && N && K && (!w || ldw < K)) ||
+        (dw && M && K && (!x || ldx < K))) return SMLVM_ERR_INVALID;
     const hipStream_t stream = (hipStream_t)stream_;
-    const int64_t need = (n + 2047) / 2048;
-    const dim3 grid((unsigned)(need < 16384 ? need : 16384));
-    const int aligned = aligned16(dy) && aligned16(h) && aligned16(dh);
-#define ACT_BWD(T) hipLaunchKernelGGL((act_bwd_kernel<T>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
-                                      static_cast<const T*>(h), static_cast<T*>(dh), n, act, aligned)
-    if (kind == SMLVM_F32) ACT_BWD(float);
-    else if (kind == SMLVM_F16) ACT_BWD(f16_t);
-    else ACT_BWD(bf16_t);
+    char* ws = static_cast<char*>(workspace);
+    if (act && some) {
+        const size_t bytes = act_bytes(kind, M, N);
+        if (!ws || workspace_bytes < bytes) return SMLVM_ERR_WORKSPACE;
+        const int64_t n = M * N, need = (n + 2047) / 2048;
+        const dim3 grid((unsigned)(need < 16384 ? need : 16384));
+        const int aligned = aligned16(dy) && aligned16(h) && aligned16(ws);
+#define ACT_BWD(T, H) hipLaunchKernelGGL((act_bwd_kernel<T, H>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
+                                         static_cast<const H*>(h), reinterpret_cast<T*>(ws), n, act, aligned)
+        if (kind == SMLVM_F32) ACT_BWD(float, float);
+        else if (kind == SMLVM_F16) ACT_BWD(f16_t, f16_t);
+        else if (h_is_y) ACT_BWD(bf16_t, bf16_t);
+        else ACT_BWD(bf16_t, f16_t);
 #undef ACT_BWD
-    return check_launch();
-}
-
-extern "C" int smlvm_linear_dx(const void* dh, int64_t ldh, const void* w, int64_t ldw, void* dx, int32_t kind, int64_t M,
-                               int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
-{
-    const int go = check_sizes(kind, M, N, K);
-    if (go <= 0) return go;
-    if (M == 0 || K == 0) return SMLVM_OK;
-    if (!dx || (N && (!dh || !w)) || (N && (ldh < N || ldw < K))) return SMLVM_ERR_INVALID;
-    GemmArgs g = {};
-    g.a = dh; g.b = w; g.lda = ldh; g.ldb = ldw; g.M = M; g.N = K; g.K = N;
-    g.out = dx; g.vec = vec4_ok(kind, K, dx, K);
-    return dispatch_gemm(kind, 1, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
-}
-
-extern "C" int smlvm_linear_dw(const void* dh, int64_t ldh, const void* x, int64_t ldx, void* dw, void* db, int32_t kind,
-                               int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream)
-{
-    const int go = check_sizes(kind, M, N, K);
-    if (go <= 0) return go;
-    if (N == 0 || K == 0) return SMLVM_OK;
-    if (!dw || (M && (!dh || !x)) || (M && (ldh < N || ldx < K))) return SMLVM_ERR_INVALID;
-    GemmArgs g = {};
-    g.a = dh; g.b = x; g.lda = ldh; g.ldb = ldx; g.M = N; g.N = K; g.K = M;
-    g.out = dw; g.vec = vec4_ok(kind, K, dw, K);
-    return dispatch_gemm(kind, 2, g, db, workspace, workspace_bytes, (hipStream_t)stream);
+        const int rc = check_launch();
+        if (rc != SMLVM_OK) return rc;
+        dy = ws;
+        ws += bytes;
+        workspace_bytes -= bytes;
+    }
+    int rc = SMLVM_OK;
+    if (dx && M && K) {
+        GemmArgs g = {};
+        g.a = dy; g.b = w; g.lda = ldy; g.ldb = ldw; g.M = M; g.N = K; g.K = N;
+        g.out = dx; g.vec = vec4_ok(kind, K, dx, K);
+        rc = dispatch_gemm(kind, 1, g, nullptr, ws, workspace_bytes, stream);
+    }
+    if (rc == SMLVM_OK && N && (K ? dw != nullptr : db != nullptr)) {
+        GemmArgs g = {};
+        g.a = dy; g.b = x; g.lda = ldy; g.ldb = ldx; g.M = N; g.N = K; g.K = M;
+        g.out = dw; g.vec = vec4_ok(kind, K, dw, K);
+        rc = dispatch_gemm(kind, 2, g, db, ws, workspace_bytes, stream);
+    }
+    return rc;
 }

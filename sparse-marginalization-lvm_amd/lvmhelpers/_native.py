@@ -35,7 +35,7 @@ ABI_SYMBOLS = [
     "smlvm_adamw_step",
     "smlvm_token_logprobs_fwd", "smlvm_token_logprobs_bwd", "smlvm_policy_loss_workspace_bytes", "smlvm_policy_loss",
     "smlvm_stream_capture_id",
-    "smlvm_linear_workspace_bytes", "smlvm_linear_fwd", "smlvm_linear_act_bwd", "smlvm_linear_dx", "smlvm_linear_dw",
+    "smlvm_linear_fwd_workspace_bytes", "smlvm_linear_bwd_workspace_bytes", "smlvm_linear_fwd", "smlvm_linear_bwd",
 ]
 
 
@@ -67,8 +67,10 @@ def lib():
         L.smlvm_lowrank_ce_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.smlvm_lowrank_ce_bwd_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32,
                                                            ctypes.c_int32, ctypes.c_int32]
-        L.smlvm_linear_workspace_bytes.restype = ctypes.c_size_t
-        L.smlvm_linear_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
+        L.smlvm_linear_fwd_workspace_bytes.restype = ctypes.c_size_t
+        L.smlvm_linear_fwd_workspace_bytes.argtypes = [ctypes.c_int32] + [ctypes.c_int64] * 3
+        L.smlvm_linear_bwd_workspace_bytes.restype = ctypes.c_size_t
+        L.smlvm_linear_bwd_workspace_bytes.argtypes = [ctypes.c_int32] * 2 + [ctypes.c_int64] * 3
         L.smlvm_policy_loss_workspace_bytes.restype = ctypes.c_size_t
         L.smlvm_policy_loss_workspace_bytes.argtypes = [ctypes.c_int64]
         if L.smlvm_abi_version() != 2:
@@ -770,11 +772,6 @@ def _rows(t, width):
     return t, max(t.stride(0), width)
 
 
-def _linear_workspace(kind, M, N, K, dev):
-    nbytes = lib().smlvm_linear_workspace_bytes(kind, M, N, K)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None, ctypes.c_size_t(nbytes)
-
-
 def linear_fwd(x, w, bias, residual, act, want_pre):
     """x [M,K], w [N,K], bias [N] or None, residual [M,N] or None, all of one type on one GPU ->
     (y [M,N], pre [M,N] or None)."""
@@ -786,44 +783,33 @@ def linear_fwd(x, w, bias, residual, act, want_pre):
         residual, ldr = _rows(residual, N)
     kind = KINDS[x.dtype]
     y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    pre = torch.empty_like(y) if want_pre else None
-    ws, nbytes = _linear_workspace(kind, M, N, K, x.device)
+    pre = torch.empty((M, N), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device) if want_pre else None
+    nbytes = lib().smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     with _on(x.device):
         _check(lib().smlvm_linear_fwd(_p(x), _i64(ldx), _p(w), _i64(ldw), _p(bias), _p(residual), _i64(ldr), _p(y), _p(pre),
-                                      _i32(kind), _i32(act), _i64(M), _i64(N), _i64(K), _p(ws), nbytes, _stream()),
-               "smlvm_linear_fwd")
+                                      _i32(kind), _i32(act), _i64(M), _i64(N), _i64(K), _p(ws),
+                                      ctypes.c_size_t(nbytes), _stream()), "smlvm_linear_fwd")
     return y, pre
 
 
-def linear_bwd(dy, h, x, w, act, want_dx, want_dw, want_db):
-    """dy [M,N], h = pre of linear_fwd (None for act 0) -> (dx, dw, db), each None unless wanted."""
+def linear_bwd(dy, h, h_is_y, x, w, act, want_dx, want_dw, want_db):
+    """dy [M,N], h = pre of linear_fwd, or y (h_is_y: relu without a residual), None for act 0 ->
+    (dx, dw, db), each None unless wanted."""
     (M, K), N = x.shape, w.shape[0]
-    dev, kind = x.device, KINDS[x.dtype]
-    dx = dw = db = None
+    dev, dt, kind = x.device, x.dtype, KINDS[x.dtype]
+    dy, ldy = (dy.contiguous(), N) if act else _rows(dy, N)
+    x, ldx = _rows(x, K)
+    w, ldw = _rows(w, K)
+    dx = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
+    dw = torch.empty((N, K), dtype=dt, device=dev) if want_dw or want_db else None
+    db = torch.empty(N, dtype=dt, device=dev) if want_db else None
+    nbytes = lib().smlvm_linear_bwd_workspace_bytes(kind, act, M, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on(dev):
-        if act:
-            dy = dy.contiguous()
-            dh = torch.empty_like(dy)
-            _check(lib().smlvm_linear_act_bwd(_p(dy), _p(h), _p(dh), _i32(kind), _i32(act), _i64(M * N), _stream()),
-                   "smlvm_linear_act_bwd")
-            ldh = N
-        else:
-            dh, ldh = _rows(dy, N)
-        ws, nbytes = _linear_workspace(kind, M, N, K, dev)
-        if want_dx:
-            w, ldw = _rows(w, K)
-            dx = torch.empty((M, K), dtype=x.dtype, device=dev)
-            _check(lib().smlvm_linear_dx(_p(dh), _i64(ldh), _p(w), _i64(ldw), _p(dx), _i32(kind), _i64(M), _i64(N), _i64(K),
-                                         _p(ws), nbytes, _stream()), "smlvm_linear_dx")
-        if want_dw or want_db:
-            x, ldx = _rows(x, K)
-            dw = torch.empty((N, K), dtype=x.dtype, device=dev)
-            db = torch.empty(N, dtype=x.dtype, device=dev) if want_db else None
-            if N and K:
-                _check(lib().smlvm_linear_dw(_p(dh), _i64(ldh), _p(x), _i64(ldx), _p(dw), _p(db), _i32(kind), _i64(M),
-                                             _i64(N), _i64(K), _p(ws), nbytes, _stream()), "smlvm_linear_dw")
-            elif db is not None:        # no inputs: the bias alone
-                db.copy_(dh.sum(0))
+        _check(lib().smlvm_linear_bwd(_p(dy), _i64(ldy), _p(h), _i32(1 if h_is_y else 0), _p(x), _i64(ldx), _p(w), _i64(ldw),
+                                      _p(dx), _p(dw), _p(db), _i32(kind), _i32(act), _i64(M), _i64(N), _i64(K), _p(ws),
+                                      ctypes.c_size_t(nbytes), _stream()), "smlvm_linear_bwd")
     return dx, (dw if want_dw else None), db
 
 

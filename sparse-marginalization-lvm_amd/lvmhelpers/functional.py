@@ -262,7 +262,7 @@ def lowrank_categorical_nll(x, w, b, y):
 
 class _LinearAct(torch.autograd.Function):
     """act(x w^T + b) + r with the epilogue in the product's kernel.  For the backward the forward leaves
-    act's argument (rounded to the tensors' type; relu without a residual keeps its output instead)."""
+    act's argument (float32, or float16 next to 16-bit tensors; relu without a residual keeps its output instead)."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, act):
@@ -270,7 +270,7 @@ class _LinearAct(torch.autograd.Function):
         own_sign = act == 1 and r is None          # relu: y > 0 exactly where its argument is
         y, pre = _native.linear_fwd(x, w, b, r, act, want_pre=need and act != 0 and not own_sign)
         if need:
-            ctx.act = act
+            ctx.act, ctx.h_is_y = act, own_sign
             ctx.save_for_backward(x, w, *([y if own_sign else pre] if act else []))
         return y
 
@@ -280,7 +280,7 @@ class _LinearAct(torch.autograd.Function):
         want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
         if want_dx or want_dw or want_db:
             x, w = ctx.saved_tensors[:2]
-            dx, dw, db = _native.linear_bwd(dy, ctx.saved_tensors[2] if ctx.act else None, x, w, ctx.act, want_dx,
+            dx, dw, db = _native.linear_bwd(dy, ctx.saved_tensors[2] if ctx.act else None, ctx.h_is_y, x, w, ctx.act, want_dx,
                                             want_dw, want_db)
         return dx, dw, db, (dy if want_dr else None), None
 

@@ -44,11 +44,11 @@ def test_c_entries_check_their_arguments():
     L = _native.lib()
     i64, i32, sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
     one = ctypes.c_void_p(16)
-    big = L.smlvm_linear_workspace_bytes(0, 4, 64, 100000)
-    assert big > 0 and L.smlvm_linear_workspace_bytes(0, 4, 4, 4) >= 16      # (column sums)
-    assert L.smlvm_linear_workspace_bytes(7, 4, 4, 4) == 0
-    for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0), (0, 0, 0)):                # empty axes
-        assert L.smlvm_linear_workspace_bytes(0, *sizes) >= 0 and L.smlvm_linear_workspace_bytes(2, *sizes) >= 0
+    big = L.smlvm_linear_fwd_workspace_bytes(0, 4, 64, 100000)
+    assert big > 0 and L.smlvm_linear_bwd_workspace_bytes(0, 2, 4, 4, 4) >= 64               # (dh)
+    assert L.smlvm_linear_fwd_workspace_bytes(7, 4, 4, 4) == 0 and L.smlvm_linear_bwd_workspace_bytes(7, 0, 4, 4, 4) == 0
+    for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0), (0, 0, 0)):                                # empty axes
+        assert L.smlvm_linear_fwd_workspace_bytes(0, *sizes) >= 0 and L.smlvm_linear_bwd_workspace_bytes(2, 1, *sizes) >= 0
 
     def fwd(x=one, ldx=100000, w=one, y=one, kind=0, act=0, M=4, N=64, K=100000, ws=one, nbytes=big, r=None, ldr=64):
         return L.smlvm_linear_fwd(x, i64(ldx), w, i64(max(K, 1)), None, r, i64(ldr), y, None, i32(kind), i32(act), i64(M), i64(N),
@@ -57,8 +57,14 @@ def test_c_entries_check_their_arguments():
     assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1 and fwd(kind=3) == -1 and fwd(act=6) == -1
     assert fwd(ldx=99999) == -1 and fwd(r=one, ldr=63) == -1 and fwd(M=-1) == -1 and fwd(M=1 << 31) == -2
     assert fwd(ws=None, nbytes=0) == -4 and fwd(nbytes=1) == -4                    # the split product's partial sums
-    assert L.smlvm_linear_act_bwd(one, None, one, i32(0), i32(1), i64(4), None) == -1
-    assert L.smlvm_linear_act_bwd(None, None, None, i32(0), i32(1), i64(0), None) == 0
-    assert L.smlvm_linear_dx(None, i64(4), one, i64(4), one, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -1
-    assert L.smlvm_linear_dw(one, i64(4), one, i64(4), one, one, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -4
-    assert L.smlvm_linear_dw(one, i64(4), one, i64(4), None, None, i32(0), i64(4), i64(4), i64(4), None, sz(0), None) == -1
+
+    need = L.smlvm_linear_bwd_workspace_bytes(0, 1, 4, 4, 4)
+
+    def bwd(dy=one, ldy=4, h=one, h_is_y=0, x=one, w=one, dx=one, dw=one, db=one, act=1, M=4, ws=one, nbytes=need):
+        return L.smlvm_linear_bwd(dy, i64(ldy), h, i32(h_is_y), x, i64(4), w, i64(4), dx, dw, db, i32(0), i32(act), i64(M), i64(4),
+                                  i64(4), ws, sz(nbytes), None)
+    assert bwd(M=-1) == -1 and bwd(act=7) == -1 and bwd(dy=None) == -1 and bwd(h=None) == -1 and bwd(x=None) == -1
+    assert bwd(w=None) == -1 and bwd(dw=None) == -1 and bwd(ldy=5) == -1 and bwd(ldy=3) == -1
+    assert bwd(act=2, h_is_y=1) == -1                                                          # y stands in for relu only
+    assert bwd(ws=None) == -4 and bwd(nbytes=8) == -4
+    assert bwd(dx=None, dw=None, db=None, act=0) == 0                                          # nothing wanted
