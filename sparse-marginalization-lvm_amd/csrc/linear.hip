@@ -107,30 +107,46 @@ struct GemmArgs {
     float* colsum_part;           // not null (column a, split): fp32 sums over k of A(m, k), [splits][M]
     void* colsum;                 // not null (column a): sums over k of A(m, k), [M]
     int act;
-    int vec;                      // out, pre, res and bias may be accessed 4 elements at a time
     int tiles_m, tiles_n;
 };
 
 // ----------------------------------------------------------------------------------- epilogue
+// 8 consecutive elements, aligned to the element only; `have` of them exist
 template <class T>
-__device__ __forceinline__ void load4(const T* p, bool vec, int have, float (&x)[4])
+__device__ __forceinline__ void load8(const T* p, int have, float (&x)[8])
 {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) load_vec<T, 4>(p, x);
-        else load_vec<T, 4>(p, x);
+    if (have == 8) {
+        constexpr int P = 16 / (int)sizeof(T);
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8 / P; ++i) {
+            const u32x4 raw = reinterpret_cast<const u32x4_any*>(p)[i];
+            __builtin_memcpy(&t[i * P], &raw, 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)t[j];
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = j < have ? (float)p[j] : 0.0f;
+        for (int j = 0; j < 8; ++j) x[j] = j < have ? (float)p[j] : 0.0f;
     }
 }
 template <class T>
-__device__ __forceinline__ void store4(T* p, bool vec, int have, const float (&x)[4])
+__device__ __forceinline__ void store8(T* p, int have, const float (&x)[8])
 {
-    if (vec) {
-        store_vec<T, 4>(p, x);
+    T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = (T)x[j];
+    if (have == 8) {
+        constexpr int P = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / P; ++i) {
+            u32x4 raw;
+            __builtin_memcpy(&raw, &t[i * P], 16);
+            reinterpret_cast<u32x4_any*>(p)[i] = raw;
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (j < have) p[j] = (T)x[j];
+        for (int j = 0; j < 8; ++j) if (j < have) p[j] = t[j];
     }
 }
 
@@ -141,38 +157,37 @@ __device__ __forceinline__ void store4(T* p, bool vec, int have, const float (&x
 template <class T> struct PreOf { typedef f16_t type; };
 template <> struct PreOf<float> { typedef float type; };
 template <class T>
-__device__ __forceinline__ void store_pre(void* pre, int64_t at, bool vec, int have, const float (&x)[4])
+__device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const float (&x)[8])
 {
-    float h[4];
+    float h[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = sizeof(T) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
-    store4(static_cast<typename PreOf<T>::type*>(pre) + at, vec, have, h);
+    for (int j = 0; j < 8; ++j) h[j] = sizeof(T) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    store8(static_cast<typename PreOf<T>::type*>(pre) + at, have, h);
 }
 
-// 4 consecutive n of row m: bias, activation, residual, stores
+// 8 consecutive n of row m: bias, activation, residual, stores
 template <class T>
-__device__ __forceinline__ void finish4(const GemmArgs& g, int64_t m, int64_t n, float (&x)[4])
+__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, float (&x)[8])
 {
-    const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
-    const bool vec = g.vec && have == 4;
+    const int have = g.N - n < 8 ? (int)(g.N - n) : 8;
+    float r[8];
+    if (g.res) load8(static_cast<const T*>(g.res) + m * g.ldr + n, have, r);
     if (g.bias) {
-        float b[4];
-        load4(static_cast<const T*>(g.bias) + n, vec, have, b);
+        float b[8];
+        load8(static_cast<const T*>(g.bias) + n, have, b);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += b[j];
+        for (int j = 0; j < 8; ++j) x[j] += b[j];
     }
-    if (g.pre) store_pre<T>(g.pre, m * g.N + n, vec, have, x);
+    if (g.pre) store_pre<T>(g.pre, m * g.N + n, have, x);
     if (g.act != kNone) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = act_f<sizeof(T) == 2>(g.act, x[j]);
+        for (int j = 0; j < 8; ++j) x[j] = act_f<sizeof(T) == 2>(g.act, x[j]);
     }
     if (g.res) {
-        float r[4];
-        load4(static_cast<const T*>(g.res) + m * g.ldr + n, vec, have, r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += r[j];
+        for (int j = 0; j < 8; ++j) x[j] += r[j];
     }
-    store4(static_cast<T*>(g.out) + m * g.N + n, vec, have, x);
+    store8(static_cast<T*>(g.out) + m * g.N + n, have, x);
 }
 
 // ------------------------------------------------------------------------------------- staging
@@ -483,29 +498,37 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
         }
     }
 
-    const int64_t nb = n0 + nw + ((lane >> 4) << 2), mb = m0 + mw + (lane & 15);
+    // 16 rows at a time through the wave's own part of the LDS: a lane holds 4 n of one row, and stores 8 of
+    // another, so that a row's stores fill whole cache lines.  (Rows 16 bytes apart in bank: no conflicts.)
+    constexpr int COLS = BN / WN, PITCH = COLS + 4, PER_ROW = COLS / 8;
+    static_assert(WM * WN * 16 * PITCH * 4 <= (DIRECT ? 2 : 1) * STAGE, "epilogue tile");
+    __syncthreads();
+    float* const own = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int64_t m = mb + i * 16;
-        if (m >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t n = nb + j * 16;
-            if (n >= g.N) continue;
-            float x[4] = {acc[i][j].x, acc[i][j].y, acc[i][j].z, acc[i][j].w};
-            if (g.part) {
-                const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
-                store4(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N % 4 == 0, have, x);
-            } else {
-                finish4<T>(g, m, n, x);
-            }
-        }
         if constexpr (ACOL) {
-            if (colsum && lane < 16 && i / FS == wave % WN) {
+            const int64_t m = m0 + mw + i * 16 + lane;
+            if (colsum && lane < 16 && m < g.M && i / FS == wave % WN) {
                 if (g.colsum_part) g.colsum_part[(int64_t)blockIdx.z * g.M + m] = sums[i % FS].x;
                 else static_cast<T*>(g.colsum)[m] = (T)sums[i % FS].x;
             }
         }
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            *reinterpret_cast<f32x4*>(own + (lane & 15) * PITCH + j * 16 + ((lane >> 4) << 2)) = acc[i][j];
+        wave_lds_sync();
+#pragma unroll
+        for (int v = 0; v < 16 * PER_ROW / 64; ++v) {
+            const int row = (v * 64 + lane) / PER_ROW, col = ((v * 64 + lane) % PER_ROW) * 8;
+            float x[8];
+            load_vec<float, 8>(own + row * PITCH + col, x);
+            const int64_t m = m0 + mw + i * 16 + row, n = n0 + nw + col;
+            if (m < g.M && n < g.N) {
+                if (g.part) store8(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N - n < 8 ? (int)(g.N - n) : 8, x);
+                else finish8<T>(g, m, n, x);
+            }
+        }
+        wave_lds_sync();
     }
 }
 
@@ -522,18 +545,18 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits,
         static_cast<T*>(g.colsum)[m] = (T)s;
         return;
     }
-    const int64_t per_row = (g.N + 3) / 4, total = g.M * per_row;
+    const int64_t per_row = (g.N + 7) / 8, total = g.M * per_row;
     for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
-        const int64_t m = v / per_row, n = (v - m * per_row) * 4;
-        const int have = g.N - n < 4 ? (int)(g.N - n) : 4;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int64_t m = v / per_row, n = (v - m * per_row) * 8;
+        const int have = g.N - n < 8 ? (int)(g.N - n) : 8;
+        float x[8] = {};
         for (int z = 0; z < splits; ++z) {
-            float y[4];
-            load4<float>(g.part + ((int64_t)z * g.M + m) * g.N + n, g.N % 4 == 0, have, y);
+            float y[8];
+            load8<float>(g.part + ((int64_t)z * g.M + m) * g.N + n, have, y);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] += y[j];
+            for (int j = 0; j < 8; ++j) x[j] += y[j];
         }
-        finish4<T>(g, m, n, x);
+        finish8<T>(g, m, n, x);
     }
 }
 
@@ -637,7 +660,7 @@ static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size
     else if (layout == 1) launch_gemm<T, false, true>(p, direct, g, stream);
     else launch_gemm<T, true, true>(p, direct, g, stream);
     if (p.splits > 1) {
-        const int64_t want = (g.M * ((g.N + 3) / 4) + 255) / 256;
+        const int64_t want = (g.M * ((g.N + 7) / 8) + 255) / 256;
         const int blocks = (int)(want < 8192 ? want : 8192);
         const int64_t sums = colsum ? (g.M + 255) / 256 : 0;
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + sums)), dim3(256), 0, stream, g, p.splits, blocks);
@@ -661,12 +684,6 @@ static size_t workspace_of(int kind, int64_t M, int64_t N, int64_t K, bool colsu
         if (need > most) most = need;
     }
     return most * sizeof(float);
-}
-
-static bool vec4_ok(int kind, int64_t N, const void* p, int64_t ld)
-{
-    const uintptr_t mask = 4 * kind_bytes(kind) - 1;
-    return !p || (((uintptr_t)p & mask) == 0 && ld % 4 == 0 && N % 4 == 0);
 }
 
 // dh, in front of the products' partial sums
@@ -708,7 +725,6 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
     GemmArgs g = {};
     g.a = x; g.b = w; g.lda = ldx; g.ldb = ldw; g.M = M; g.N = N; g.K = K;
     g.out = y; g.bias = bias; g.res = residual; g.ldr = ldr; g.pre = pre; g.act = act;
-    g.vec = vec4_ok(kind, N, y, N) && vec4_ok(kind, N, pre, N) && vec4_ok(kind, N, residual, ldr) && vec4_ok(kind, N, bias, 0);
     return dispatch_gemm(kind, 0, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -747,13 +763,13 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
     if (dx && M && K) {
         GemmArgs g = {};
         g.a = dy; g.b = w; g.lda = ldy; g.ldb = ldw; g.M = M; g.N = K; g.K = N;
-        g.out = dx; g.vec = vec4_ok(kind, K, dx, K);
+        g.out = dx;
         rc = dispatch_gemm(kind, 1, g, nullptr, ws, workspace_bytes, stream);
     }
     if (rc == SMLVM_OK && N && (K ? dw != nullptr : db != nullptr)) {
         GemmArgs g = {};
         g.a = dy; g.b = x; g.lda = ldy; g.ldb = ldx; g.M = N; g.N = K; g.K = M;
-        g.out = dw; g.vec = vec4_ok(kind, K, dw, K);
+        g.out = dw;
         rc = dispatch_gemm(kind, 2, g, db, ws, workspace_bytes, stream);
     }
     return rc;
