@@ -167,9 +167,9 @@ __device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const
 
 // 8 consecutive n of row m: bias, activation, residual, stores
 template <class T>
-__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, float (&x)[8])
+__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, float (&x)[8], int most = 8)
 {
-    const int have = g.N - n < 8 ? (int)(g.N - n) : 8;
+    const int have = g.N - n < most ? (int)(g.N - n) : most;
     float r[8];
     if (g.res) load8(static_cast<const T*>(g.res) + m * g.ldr + n, have, r);
     if (g.bias) {
@@ -307,28 +307,70 @@ struct Through {
     static constexpr int kVecs = (int)sizeof(T) / 2;                    // 16-byte loads per 8 elements
     static_assert(Tl::kSlots % THREADS == 0, "whole slots per thread");
     u32x4 held[kEach][kVecs];
+    const T* from[kEach];                                               // the slot's elements at the current k
+    int64_t step;
 
-    __device__ __forceinline__ void load(const T* src, int64_t ld, int64_t first, int64_t extent, int64_t k0, int64_t k_end)
+    __device__ __forceinline__ void init(const T* src, int64_t ld, int64_t first, int64_t k0)
     {
+        step = COL ? BK * ld : BK;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             int row, at;
             Tl::source(i * THREADS + threadIdx.x, row, at);
-            const int64_t r = COL ? k0 + row : first + row, c = COL ? first + at : k0 + at;
-            const int64_t r_end = COL ? k_end : extent, c_end = COL ? extent : k_end;
-            const T* p = src + r * ld + c;
+            from[i] = COL ? src + (k0 + row) * ld + first + at : src + (first + row) * ld + k0 + at;
+        }
+    }
+    // `rows`: what is left of the matrix' m (n), `k_left` of this part's k, `k_all` of the matrix'; then on to the
+    // next k tile.  At an edge a slot that ends behind its row is read whole where another stored row
+    // follows (the elements too many are of an m nobody stores, or a k that is cleared here), element by
+    // element in the last one.
+    __device__ __forceinline__ void load(int64_t rows, int64_t k_left, int64_t k_all)
+    {
+        if (rows >= ROWS && k_left >= BK) {                             // (uniform)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+                for (int v = 0; v < kVecs; ++v) held[i][v] = reinterpret_cast<const u32x4_any*>(from[i])[v];
+                from[i] += step;
+            }
+            return;
+        }
+        const int r_end = (int)(COL ? (k_left < BK ? k_left : BK) : (rows < ROWS ? rows : ROWS));
+        const int c_end = (int)(COL ? (rows < ROWS ? rows : ROWS) : (k_left < BK ? k_left : BK));
+        const int64_t r_all = COL ? k_all : rows;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            int row, at;
+            Tl::source(i * THREADS + threadIdx.x, row, at);
+            const bool in = row < r_end && at < c_end, whole = at + 8 <= c_end || row + 1 < r_all;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) held[i][v] = u32x4{0u, 0u, 0u, 0u};
-            if (r < r_end) {
-                if (c + 8 <= c_end) {
+            if (in && whole) {
 #pragma unroll
-                    for (int v = 0; v < kVecs; ++v) held[i][v] = reinterpret_cast<const u32x4_any*>(p)[v];
-                } else if (c < c_end) {
-                    T t[8] = {};
+                for (int v = 0; v < kVecs; ++v) held[i][v] = reinterpret_cast<const u32x4_any*>(from[i])[v];
+            }
+            if (in && !whole) {
+                T t[8] = {};
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) if (c + j < c_end) t[j] = p[j];
-                    __builtin_memcpy(held[i], t, 8 * sizeof(T));
-                }
+                for (int j = 0; j < 8; ++j) if (at + j < c_end) t[j] = from[i][j];
+                __builtin_memcpy(held[i], t, 8 * sizeof(T));
+            }
+            from[i] += step;
+        }
+        if (!COL && k_left < BK) {                                      // (uniform) clear the k behind the last one
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                int row, at;
+                Tl::source(i * THREADS + threadIdx.x, row, at);
+                const int have = c_end - at;
+#pragma unroll
+                for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int e = (v * 4 + j) * 4 / (int)sizeof(T);  // the word's first element
+                        if constexpr (sizeof(T) == 4) held[i][v][j] = e < have ? held[i][v][j] : 0u;
+                        else held[i][v][j] &= e + 1 < have ? 0xFFFFFFFFu : e < have ? 0xFFFFu : 0u;
+                    }
             }
         }
     }
@@ -481,9 +523,11 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
     } else {
         Through<T, BM, BK, ACOL, THREADS> sa;
         Through<T, BN, BK, BCOL, THREADS> sb;
+        sa.init(a, g.lda, m0, k_begin);
+        sb.init(b, g.ldb, n0, k_begin);
         if (steps > 0) {
-            sa.load(a, g.lda, m0, g.M, k_begin, k_end);
-            sb.load(b, g.ldb, n0, g.N, k_begin, k_end);
+            sa.load(g.M - m0, k_end - k_begin, g.K - k_begin);
+            sb.load(g.N - n0, k_end - k_begin, g.K - k_begin);
         }
         for (int64_t s = 0; s < steps; ++s) {
             __syncthreads();                                             // (the last tile has been read)
@@ -491,8 +535,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
             sb.store(lds + PLANES * TA::kBytes);
             __syncthreads();
             if (s + 1 < steps) {
-                sa.load(a, g.lda, m0, g.M, k_begin + (s + 1) * BK, k_end);
-                sb.load(b, g.ldb, n0, g.N, k_begin + (s + 1) * BK, k_end);
+                const int64_t left = k_end - k_begin - (s + 1) * BK, all = g.K - k_begin - (s + 1) * BK;
+                sa.load(g.M - m0, left, all);
+                sb.load(g.N - n0, left, all);
             }
             compute(lds);
         }
@@ -529,6 +574,76 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
             }
         }
         wave_lds_sync();
+    }
+}
+
+// Few rows (M <= kFewRows): bound by reading w once.  A wave owns two rows of w, its lanes go along k 16 bytes at a
+// time, x comes out of the caches; the sums are joined across the lanes at the end.  One launch, where the tiled
+// kernel needs a split over k and a join: [1 x 4096] [4096 x 4096]^T bf16 takes 8.6 us against 10.7.
+constexpr int kFewRows = 4;
+template <class T, int MR>
+__global__ __launch_bounds__(256) void few_rows_kernel(const GemmArgs g)
+{
+    constexpr int P = 16 / (int)sizeof(T), NW = 2, U = MR <= 2 ? 4 : 2;
+    const int lane = threadIdx.x & 63;
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * NW;
+    if (n0 >= g.N) return;
+    const T* const x = static_cast<const T*>(g.a);
+    const T* w[NW];
+#pragma unroll
+    for (int c = 0; c < NW; ++c) w[c] = static_cast<const T*>(g.b) + (n0 + c < g.N ? n0 + c : n0) * g.ldb;
+    float acc[MR][NW] = {};
+    const int64_t whole = g.K / P * P;
+    int64_t k = (int64_t)lane * P;
+    auto step = [&](const u32x4 (&wv)[NW], int64_t at) {
+        T wt[NW][P];
+#pragma unroll
+        for (int c = 0; c < NW; ++c) __builtin_memcpy(wt[c], &wv[c], 16);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            const u32x4 xv = *reinterpret_cast<const u32x4_any*>(x + m * g.lda + at);
+            T xt[P];
+            __builtin_memcpy(xt, &xv, 16);
+#pragma unroll
+            for (int c = 0; c < NW; ++c)
+#pragma unroll
+                for (int j = 0; j < P; ++j) acc[m][c] = fmaf((float)xt[j], (float)wt[c][j], acc[m][c]);
+        }
+    };
+    for (; k + (U - 1) * 64 * P < whole; k += U * 64 * P) {
+        u32x4 wv[U][NW];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < NW; ++c) wv[u][c] = *reinterpret_cast<const u32x4_any*>(w[c] + k + u * 64 * P);
+#pragma unroll
+        for (int u = 0; u < U; ++u) step(wv[u], k + u * 64 * P);
+    }
+    for (; k < whole; k += 64 * P) {
+        u32x4 wv[NW];
+#pragma unroll
+        for (int c = 0; c < NW; ++c) wv[c] = *reinterpret_cast<const u32x4_any*>(w[c] + k);
+        step(wv, k);
+    }
+    if (whole + lane < g.K) {
+        const int64_t at = whole + lane;
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+            for (int c = 0; c < NW; ++c) acc[m][c] = fmaf((float)x[m * g.lda + at], (float)w[c][at], acc[m][c]);
+    }
+    float mine = 0.0f;                                                   // lane m * NW + c keeps sum (m, c)
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < NW; ++c) {
+            const float sum = group_reduce<64>(acc[m][c], OpSum{});
+            if (lane == m * NW + c) mine = sum;
+        }
+    const int64_t n = n0 + lane % NW;
+    if (lane < MR * NW && n < g.N) {
+        float one[8] = {mine};
+        finish8<T>(g, lane / NW, n, one, 1);
     }
 }
 
@@ -583,28 +698,42 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, 
 // -------------------------------------------------------------------------------------- host side
 struct Plan { int bm, bn, splits; int64_t k_split; };
 
-// Tile and split: the largest tile that still gives every CU a workgroup; the smallest one otherwise,
-// with the k range split until there are some two workgroups per CU (each keeping 4 k tiles).
+// Tile and split of k by the estimated time of each combination.  A workgroup costs `fixed` us plus, per k
+// tile, its own latency or its share of the CU, whichever is more; a split adds the join's launch and
+// its traffic.  The numbers are fits to products timed alone (us): 2048^3 bf16 with 64 / 128 / 256 tiles
+// 25.6 / 26.5 / 57.8; [53000 x 3920]^T [53000 x 128] fp32 with 64 tiles in 5 parts 499, with 128 tiles in 16
+// parts 344; [200 x 4000] [4000 x 4000]^T fp32 with 64 tiles whole 134, in 4 parts 63, with 128 tiles in 8 parts 53; [1 x 4096] [4096 x 4096]^T bf16 with 64 tiles whole 31, in 8 parts 10.7.
 static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
 {
-    const int64_t bk = kind == SMLVM_F32 ? 32 : 64;
-    auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    Plan p = {64, 64, 1, 0};
-    if (direct && tiles(256) >= 256) p.bm = p.bn = 256;
-    else if (tiles(128) >= 200) p.bm = p.bn = 128;
-    const int64_t have = tiles(p.bm);
-    int64_t splits = 1;
-    if (have > 0 && have < 256) {
-        splits = (512 + have - 1) / have;
-        const int64_t most = K / (4 * bk);
-        if (splits > most) splits = most;
-        if (splits > 64) splits = 64;
-        if (splits < 1) splits = 1;
+    struct Tile { int size, slots; double fixed, latency, share; };
+    static const Tile kF32[] = {{128, 2, 5.0, 1.80, 1.14}, {64, 4, 3.0, 0.95, 0.45}};
+    static const Tile kDirect[] = {{256, 1, 14.0, 1.75, 1.75}, {128, 2, 5.0, 0.75, 0.60}, {64, 5, 2.5, 0.42, 0.18}};
+    static const Tile kThrough[] = {{128, 2, 6.0, 1.50, 0.95}, {64, 5, 3.0, 0.85, 0.27}};
+    const Tile* const set = kind == SMLVM_F32 ? kF32 : direct ? kDirect : kThrough;
+    const int sizes = kind == SMLVM_F32 ? 2 : direct ? 3 : 2;
+    const int64_t bk = kind == SMLVM_F32 ? 32 : 64, k_tiles = (K + bk - 1) / bk;
+    Plan best = {64, 64, 1, bk};
+    double least = 1e300;
+    for (int i = 0; i < sizes; ++i) {
+        const Tile& t = set[i];
+        const double tiles = (double)((M + t.size - 1) / t.size) * (double)((N + t.size - 1) / t.size);
+        for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits / 2) {
+            const int64_t per = k_tiles > 0 ? (k_tiles + splits - 1) / splits : 1;
+            if (splits > 1 && per < 4) break;
+            const double each_cu = ceil(tiles * splits / 256.0);
+            const double at_once = each_cu < t.slots ? each_cu : t.slots;
+            const double step = t.latency > at_once * t.share ? t.latency : at_once * t.share;
+            double time = ceil(each_cu / at_once) * (t.fixed + (double)per * step);
+            if (splits > 1) time += 4.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
+            if (time < least) {
+                least = time;
+                best.bm = best.bn = t.size;
+                best.k_split = per * bk;
+                best.splits = (int)(k_tiles > 0 ? (k_tiles + per - 1) / per : 1);
+            }
+        }
     }
-    const int64_t per = ((K + splits - 1) / splits + bk - 1) / bk * bk;
-    p.k_split = per > 0 ? per : bk;
-    p.splits = (int)(K > 0 ? (K + p.k_split - 1) / p.k_split : 1);
-    return p;
+    return best;
 }
 
 static bool direct_ok(int kind, const void* p, int64_t ld, int64_t contiguous)
@@ -636,11 +765,27 @@ static void launch_gemm(const Plan& p, bool direct, GemmArgs& g, hipStream_t str
 #undef GEMM
 }
 
+template <class T>
+static void launch_few_rows(const GemmArgs& g, hipStream_t stream)
+{
+    const dim3 grid((unsigned)((g.N + 7) / 8));
+    switch (g.M) {
+        case 1: hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(256), 0, stream, g); break;
+        case 2: hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(256), 0, stream, g); break;
+        case 3: hipLaunchKernelGGL((few_rows_kernel<T, 3>), grid, dim3(256), 0, stream, g); break;
+        default: hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, dim3(256), 0, stream, g); break;
+    }
+}
+
 // layout 0: rows x rows, 1: rows x columns, 2: columns x columns
 template <class T>
 static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
 {
     const int kind = KindOf<T>::value;
+    if (layout == 0 && g.M <= kFewRows) {
+        launch_few_rows<T>(g, stream);
+        return check_launch();
+    }
     const bool direct = direct_ok(kind, g.a, g.lda, layout == 2 ? g.M : g.K) && direct_ok(kind, g.b, g.ldb, layout ? g.N : g.K);
     const Plan p = plan(kind, g.M, g.N, g.K, direct);
     if ((double)((g.M + p.bm - 1) / p.bm) * (double)((g.N + p.bn - 1) / p.bn) > 2147483647.0) return SMLVM_ERR_UNSUPPORTED;
@@ -703,7 +848,7 @@ using namespace smlvm;
 
 extern "C" size_t smlvm_linear_fwd_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K)
 {
-    return check_sizes(kind, M, N, K) == 1 ? workspace_of(kind, M, N, K, false) : 0;
+    return check_sizes(kind, M, N, K) == 1 && M > kFewRows ? workspace_of(kind, M, N, K, false) : 0;
 }
 
 extern "C" size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, int64_t M, int64_t N, int64_t K)

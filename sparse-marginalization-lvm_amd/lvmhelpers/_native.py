@@ -67,12 +67,22 @@ def lib():
         L.smlvm_lowrank_ce_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.smlvm_lowrank_ce_bwd_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32,
                                                            ctypes.c_int32, ctypes.c_int32]
-        L.smlvm_linear_fwd_workspace_bytes.restype = ctypes.c_size_t
-        L.smlvm_linear_fwd_workspace_bytes.argtypes = [ctypes.c_int32] + [ctypes.c_int64] * 3
-        L.smlvm_linear_bwd_workspace_bytes.restype = ctypes.c_size_t
-        L.smlvm_linear_bwd_workspace_bytes.argtypes = [ctypes.c_int32] * 2 + [ctypes.c_int64] * 3
-        L.smlvm_policy_loss_workspace_bytes.restype = ctypes.c_size_t
-        L.smlvm_policy_loss_workspace_bytes.argtypes = [ctypes.c_int64]
+        # (with argtypes plain numbers are passed: a wrapper object per argument costs 0.15 us, 20 and more a call)
+        v, l, i, f, d, z, u = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double,
+                               ctypes.c_size_t, ctypes.c_uint32)
+        for name, restype, argtypes in (
+                ("linear_fwd_workspace_bytes", z, [i, l, l, l]),
+                ("linear_bwd_workspace_bytes", z, [i, i, l, l, l]),
+                ("linear_fwd", i, [v, l, v, l, v, v, l, v, v, i, i, l, l, l, v, z, v]),
+                ("linear_bwd", i, [v, l, v, i, v, l, v, l, v, v, v, i, i, l, l, l, v, z, v]),
+                ("token_logprobs_fwd", i, [v, i, l, l, v, v, v, v, v, l, l, l, v]),
+                ("token_logprobs_bwd", i, [v, i, l, l, v, v, v, v, v, v, i, v, l, l, l, v]),
+                ("policy_loss_workspace_bytes", z, [l]),
+                ("policy_loss", i, [v, i, l, l, v, v, v, v, v, f, f, f, f, i, v, v, v, v, v, v, v, v, v, l, l, l, v, z, v]),
+                ("stream_capture_id", i, [v, v]),
+                ("adamw_step", i, [v, i, i, i, i, d, d, f, f, v, f, u, v, v])):
+            fn = getattr(L, "smlvm_" + name)
+            fn.restype, fn.argtypes = restype, argtypes
         if L.smlvm_abi_version() != 2:
             raise NativeError("libsparsemarg_hip.so: ABI version mismatch")
         _lib = L
@@ -102,6 +112,16 @@ def _stream():
     if _raw_stream is not None and _raw_device is not None:
         return ctypes.c_void_p(_raw_stream(_raw_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _stream_ptr():
+    if _raw_stream is not None and _raw_device is not None:
+        return _raw_stream(_raw_device())
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class _Noop:
@@ -787,9 +807,9 @@ def linear_fwd(x, w, bias, residual, act, want_pre):
     nbytes = lib().smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     with _on(x.device):
-        _check(lib().smlvm_linear_fwd(_p(x), _i64(ldx), _p(w), _i64(ldw), _p(bias), _p(residual), _i64(ldr), _p(y), _p(pre),
-                                      _i32(kind), _i32(act), _i64(M), _i64(N), _i64(K), _p(ws),
-                                      ctypes.c_size_t(nbytes), _stream()), "smlvm_linear_fwd")
+        _check(lib().smlvm_linear_fwd(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, _ptr(y), _ptr(pre),
+                                      kind, act, M, N, K, _ptr(ws),
+                                      nbytes, _stream_ptr()), "smlvm_linear_fwd")
     return y, pre
 
 
@@ -807,9 +827,9 @@ def linear_bwd(dy, h, h_is_y, x, w, act, want_dx, want_dw, want_db):
     nbytes = lib().smlvm_linear_bwd_workspace_bytes(kind, act, M, N, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on(dev):
-        _check(lib().smlvm_linear_bwd(_p(dy), _i64(ldy), _p(h), _i32(1 if h_is_y else 0), _p(x), _i64(ldx), _p(w), _i64(ldw),
-                                      _p(dx), _p(dw), _p(db), _i32(kind), _i32(act), _i64(M), _i64(N), _i64(K), _p(ws),
-                                      ctypes.c_size_t(nbytes), _stream()), "smlvm_linear_bwd")
+        _check(lib().smlvm_linear_bwd(_ptr(dy), ldy, _ptr(h), 1 if h_is_y else 0, _ptr(x), ldx, _ptr(w), ldw,
+                                      _ptr(dx), _ptr(dw), _ptr(db), kind, act, M, N, K, _ptr(ws),
+                                      nbytes, _stream_ptr()), "smlvm_linear_bwd")
     return dx, (dw if want_dw else None), db
 
 
@@ -827,7 +847,7 @@ def _need_rows(logits):
 
 
 def _rows_args(logits, actions, mask):
-    return (_p(logits), _i32(KINDS[logits.dtype]), _i64(logits.stride(0)), _i64(logits.stride(1)), _p(actions), _p(mask))
+    return (_ptr(logits), KINDS[logits.dtype], logits.stride(0), logits.stride(1), _ptr(actions), _ptr(mask))
 
 
 def token_logprobs_fwd(logits, actions, mask=None, want_stats=True):
@@ -839,8 +859,8 @@ def token_logprobs_fwd(logits, actions, mask=None, want_stats=True):
     entropy = torch.empty_like(logp)
     stats = torch.empty((B, T, 3), dtype=torch.float32, device=dev) if want_stats else None
     with _on(dev):
-        _check(lib().smlvm_token_logprobs_fwd(*_rows_args(logits, actions, mask), _p(logp), _p(entropy), _p(stats),
-                                              _i64(B), _i64(T), _i64(V), _stream()), "smlvm_token_logprobs_fwd")
+        _check(lib().smlvm_token_logprobs_fwd(*_rows_args(logits, actions, mask), _ptr(logp), _ptr(entropy), _ptr(stats),
+                                              B, T, V, _stream_ptr()), "smlvm_token_logprobs_fwd")
     return logp, entropy, stats
 
 
@@ -853,9 +873,9 @@ def token_logprobs_bwd(logits, actions, mask, stats, c, h, g=None, out=None):
     if out is None:
         out = torch.empty((B, T, V), dtype=logits.dtype, device=logits.device)
     with _on(logits.device):
-        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), _p(stats), _p(c), _p(h),
-                                              _p(g), _i32(1 if keep else 0), _p(out), _i64(B), _i64(T), _i64(V),
-                                              _stream()), "smlvm_token_logprobs_bwd")
+        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), _ptr(stats), _ptr(c), _ptr(h),
+                                              _ptr(g), 1 if keep else 0, _ptr(out), B, T, V,
+                                              _stream_ptr()), "smlvm_token_logprobs_bwd")
     return out
 
 
@@ -879,10 +899,10 @@ def policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low,
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         _check(lib().smlvm_policy_loss(
-            *_rows_args(logits, actions, mask), _p(old_logp), _p(advantages), _p(ref_logp), _f32(clip_low),
-            _f32(clip_high), _f32(kl_coeff), _f32(entropy_coeff), _i32(1 if mean else 0), _p(out["loss"]),
-            _p(out["logp"]), _p(out["entropy"]), _p(out["kl"]), _p(out["clipped"]), _p(out["stats"]), _p(out["c"]),
-            _p(out["h"]), _p(out["dlogits"]), _i64(B), _i64(T), _i64(V), _p(ws), ctypes.c_size_t(nbytes), _stream()),
+            *_rows_args(logits, actions, mask), _ptr(old_logp), _ptr(advantages), _ptr(ref_logp), clip_low,
+            clip_high, kl_coeff, entropy_coeff, 1 if mean else 0, _ptr(out["loss"]),
+            _ptr(out["logp"]), _ptr(out["entropy"]), _ptr(out["kl"]), _ptr(out["clipped"]), _ptr(out["stats"]), _ptr(out["c"]),
+            _ptr(out["h"]), _ptr(out["dlogits"]), B, T, V, _ptr(ws), nbytes, _stream_ptr()),
             "smlvm_policy_loss")
     return out
 
@@ -890,7 +910,7 @@ def policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low,
 def capture_id():
     """The id of the graph capture that the current stream is part of, 0 outside one."""
     got = ctypes.c_uint64(0)
-    _check(lib().smlvm_stream_capture_id(_stream(), ctypes.byref(got)), "smlvm_stream_capture_id")
+    _check(lib().smlvm_stream_capture_id(_stream_ptr(), ctypes.byref(got)), "smlvm_stream_capture_id")
     return got.value
 
 
@@ -903,10 +923,10 @@ def adamw_step(entries, p_dtype, g_dtype, state_bits, betas, eps, lr, weight_dec
     device); lr: a number, or a float32 GPU tensor of one element; ticket: int32 [1], zero."""
     lr_dev = lr if isinstance(lr, torch.Tensor) else None
     _check(lib().smlvm_adamw_step(
-        ctypes.c_char_p(entries), _i32(len(entries) // ADAMW_ENTRY.size), _i32(KINDS[p_dtype]), _i32(KINDS[g_dtype]),
-        _i32(state_bits), ctypes.c_double(betas[0]), ctypes.c_double(betas[1]), _f32(eps),
-        _f32(0.0 if lr_dev is not None else lr), _p(lr_dev), _f32(weight_decay), ctypes.c_uint32(seed & 0xFFFFFFFF),
-        _p(ticket), _stream()), "smlvm_adamw_step")
+        entries, len(entries) // ADAMW_ENTRY.size, KINDS[p_dtype], KINDS[g_dtype],
+        state_bits, betas[0], betas[1], eps,
+        0.0 if lr_dev is not None else lr, _ptr(lr_dev), weight_decay, seed & 0xFFFFFFFF,
+        _ptr(ticket), _stream_ptr()), "smlvm_adamw_step")
 
 
 # ----------------------------------------------------------------------------------- HIP graphs

@@ -317,7 +317,11 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         residual = residual.reshape(x.shape[0], weight.shape[0])
     if bias is not None:
         bias = bias.contiguous()
-    y = _LinearAct.apply(x, weight, bias, residual, act)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        y = _LinearAct.apply(x, weight, bias, residual, act)
+    else:
+        y = _native.linear_fwd(x, weight, bias, residual, act, False)[0]
     return y if len(out_shape) == 2 else y.view(out_shape)
 
 
@@ -427,7 +431,11 @@ def token_logprobs(logits, actions, mask=None):
     give 0.  Leading axes may be strided (a shifted slice of a model's output is not copied)."""
     rows, act = _policy_rows(logits, actions, "token_logprobs")
     lead = logits.shape[:-1]
-    logp, entropy = _TokenLogprobs.apply(rows, act, _row_mask(mask, lead, rows, "token_logprobs"))
+    mask = _row_mask(mask, lead, rows, "token_logprobs")
+    if torch.is_grad_enabled() and rows.requires_grad:
+        logp, entropy = _TokenLogprobs.apply(rows, act, mask)
+    else:
+        logp, entropy, _ = _native.token_logprobs_fwd(rows, act, mask, want_stats=False)
     return logp.view(lead), entropy.view(lead)
 
 

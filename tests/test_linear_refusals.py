@@ -44,13 +44,13 @@ def test_c_entries_check_their_arguments():
     L = _native.lib()
     i64, i32, sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
     one = ctypes.c_void_p(16)
-    big = L.smlvm_linear_fwd_workspace_bytes(0, 4, 64, 100000)
+    big = L.smlvm_linear_fwd_workspace_bytes(0, 5, 64, 100000)
     assert big > 0 and L.smlvm_linear_bwd_workspace_bytes(0, 2, 4, 4, 4) >= 64               # (dh)
     assert L.smlvm_linear_fwd_workspace_bytes(7, 4, 4, 4) == 0 and L.smlvm_linear_bwd_workspace_bytes(7, 0, 4, 4, 4) == 0
     for sizes in ((0, 4, 4), (4, 0, 4), (4, 4, 0), (0, 0, 0)):                                # empty axes
         assert L.smlvm_linear_fwd_workspace_bytes(0, *sizes) >= 0 and L.smlvm_linear_bwd_workspace_bytes(2, 1, *sizes) >= 0
 
-    def fwd(x=one, ldx=100000, w=one, y=one, kind=0, act=0, M=4, N=64, K=100000, ws=one, nbytes=big, r=None, ldr=64):
+    def fwd(x=one, ldx=100000, w=one, y=one, kind=0, act=0, M=5, N=64, K=100000, ws=one, nbytes=big, r=None, ldr=64):
         return L.smlvm_linear_fwd(x, i64(ldx), w, i64(max(K, 1)), None, r, i64(ldr), y, None, i32(kind), i32(act), i64(M), i64(N),
                                   i64(K), ws, sz(nbytes), None)
     assert fwd(M=0) == 0 and fwd(N=0) == 0
