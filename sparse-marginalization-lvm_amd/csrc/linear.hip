@@ -98,7 +98,7 @@ struct GemmArgs {
     const void *a, *b;
     int64_t lda, ldb;             // elements between rows (k rows of a column operand)
     int64_t M, N, K;
-    int64_t k_split;              // k range of one blockIdx.z, a multiple of the k tile
+    int64_t k_split;              // k range of one part, a multiple of the k tile
     void* out;                    // [M][N]
     const void *bias, *res;       // nullable; res [M][N] with row stride ldr
     int64_t ldr;
@@ -406,9 +406,15 @@ struct Through {
 };
 
 // ------------------------------------------------------------------------------------ the kernel
-// BM x BN tile, WM x WN waves, DIRECT: 16-bit aligned operands.
+// BM x BN tile, WM x WN waves, DIRECT: 16-bit aligned operands.  Through registers one LDS buffer does: the next
+// tile waits in registers, and two or three workgroups per CU fill each other's gaps (two buffers of the fp32
+// planes would leave room for one).
+template <class T, int BM, int BN, bool DIRECT>
+constexpr int kLdsBytes = sizeof(T) == 4 ? 3 * (BM + BN) * 32 * 2 : (DIRECT ? 2 : 1) * (BM + BN) * 64 * 2;
+
+// tile `id` of part `part_z`
 template <class T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
+__device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z, char* lds)
 {
     constexpr int THREADS = WM * WN * 64;
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -418,16 +424,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
     using TA = Tile<BM, BK, ACOL>;
     using TB = Tile<BN, BK, BCOL>;
     constexpr int STAGE = PLANES * (TA::kBytes + TB::kBytes);
-    // Through registers one buffer does: the next tile waits in registers, and two or three workgroups per
-    // CU fill each other's gaps (two buffers of the fp32 planes would leave room for one).
-    __shared__ __attribute__((aligned(16))) char lds[(DIRECT ? 2 : 1) * STAGE];
+    static_assert(kLdsBytes<T, BM, BN, DIRECT> == (DIRECT ? 2 : 1) * STAGE, "LDS");
 
     // (wave in a scalar register: matrix instructions ignore the exec mask, so what skips one has to be a
     // scalar branch)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the 8 XCDs: give each XCD, with its own L2, one stretch of tiles, walked in
     // groups of 8 row tiles so that its neighbours share operands.
-    int id = blockIdx.x;
     const int tiles = g.tiles_m * g.tiles_n;
     {
         const int per = tiles / 8, rest = tiles % 8, xcd = id % 8, at = id / 8;
@@ -438,7 +441,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
     const int in_group = id - group * 8 * g.tiles_n;
     const int64_t m0 = (int64_t)(first_m + in_group % rows_here) * BM;
     const int64_t n0 = (int64_t)(in_group / rows_here) * BN;
-    const int64_t k_begin = (int64_t)blockIdx.z * g.k_split;
+    const int64_t k_begin = (int64_t)part_z * g.k_split;
     const int64_t k_end = g.K < k_begin + g.k_split ? g.K : k_begin + g.k_split;
     const int mw = (wave / WN) * (BM / WM), nw = (wave % WN) * (BN / WN);
     const bool colsum = ACOL && g.colsum && n0 == 0;
@@ -554,7 +557,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
         if constexpr (ACOL) {
             const int64_t m = m0 + mw + i * 16 + lane;
             if (colsum && lane < 16 && m < g.M && i / FS == wave % WN) {
-                if (g.colsum_part) g.colsum_part[(int64_t)blockIdx.z * g.M + m] = sums[i % FS].x;
+                if (g.colsum_part) g.colsum_part[(int64_t)part_z * g.M + m] = sums[i % FS].x;
                 else static_cast<T*>(g.colsum)[m] = (T)sums[i % FS].x;
             }
         }
@@ -569,11 +572,34 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
             load_vec<float, 8>(own + row * PITCH + col, x);
             const int64_t m = m0 + mw + i * 16 + row, n = n0 + nw + col;
             if (m < g.M && n < g.N) {
-                if (g.part) store8(g.part + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N - n < 8 ? (int)(g.N - n) : 8, x);
+                if (g.part) store8(g.part + ((int64_t)part_z * g.M + m) * g.N + n, g.N - n < 8 ? (int)(g.N - n) : 8, x);
                 else finish8<T>(g, m, n, x);
             }
         }
         wave_lds_sync();
+    }
+}
+
+template <class T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const GemmArgs g)
+{
+    __shared__ __attribute__((aligned(16))) char lds[kLdsBytes<T, BM, BN, DIRECT>];
+    gemm_body<T, ACOL, BCOL, BM, BN, WM, WN, DIRECT>(g, blockIdx.x, blockIdx.z, lds);
+}
+
+// A layer's two backward products in one launch, where neither fills the card by itself: [1001 x 777] with
+// [777 x 333] and [333 x 1001], fp16, 27 us one after the other.
+template <class T, bool DIRECT>
+__global__ __launch_bounds__(256) void pair_kernel(const GemmArgs dx, const GemmArgs dw, int blocks_dx)
+{
+    __shared__ __attribute__((aligned(16))) char lds[kLdsBytes<T, 64, 64, DIRECT>];
+    const int id = blockIdx.x;
+    if (id < blocks_dx) {
+        const int tiles = dx.tiles_m * dx.tiles_n;
+        gemm_body<T, false, true, 64, 64, 2, 2, DIRECT>(dx, id % tiles, id / tiles, lds);
+    } else {
+        const int tiles = dw.tiles_m * dw.tiles_n;
+        gemm_body<T, true, true, 64, 64, 2, 2, DIRECT>(dw, (id - blocks_dx) % tiles, (id - blocks_dx) / tiles, lds);
     }
 }
 
@@ -649,11 +675,13 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const GemmArgs g)
 
 // Joins the partial sums of a split product, in order, and runs the epilogue; the workgroups behind the
 // first `blocks` join the column sums.
+struct Join { int splits, blocks, sum_blocks; };
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits, int blocks)
+__device__ __forceinline__ void join_body(const GemmArgs& g, const Join& p, int id)
 {
-    if ((int)blockIdx.x >= blocks) {
-        const int64_t m = (int64_t)(blockIdx.x - blocks) * 256 + threadIdx.x;
+    const int splits = p.splits, blocks = p.blocks;
+    if (id >= blocks) {
+        const int64_t m = (int64_t)(id - blocks) * 256 + threadIdx.x;
         if (m >= g.M) return;
         float s = 0.0f;
         for (int z = 0; z < splits; ++z) s += g.colsum_part[(int64_t)z * g.M + m];
@@ -661,7 +689,7 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits,
         return;
     }
     const int64_t per_row = (g.N + 7) / 8, total = g.M * per_row;
-    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
+    for (int64_t v = (int64_t)id * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
         const int64_t m = v / per_row, n = (v - m * per_row) * 8;
         const int have = g.N - n < 8 ? (int)(g.N - n) : 8;
         float x[8] = {};
@@ -673,6 +701,15 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, int splits,
         }
         finish8<T>(g, m, n, x);
     }
+}
+
+// one product's, and behind its workgroups another's
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, const Join p, const GemmArgs g2, const Join p2)
+{
+    const int id = blockIdx.x, first = p.blocks + p.sum_blocks;
+    if (id < first) join_body<T>(g, p, id);
+    else join_body<T>(g2, p2, id - first);
 }
 
 // dh = dy act'(h), H the type h is kept in; relu may be given y in the place of h (the sign is the same).
@@ -724,7 +761,7 @@ static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
             const double at_once = each_cu < t.slots ? each_cu : t.slots;
             const double step = t.latency > at_once * t.share ? t.latency : at_once * t.share;
             double time = ceil(each_cu / at_once) * (t.fixed + (double)per * step);
-            if (splits > 1) time += 4.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
+            if (splits > 1) time += 6.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
             if (time < least) {
                 least = time;
                 best.bm = best.bn = t.size;
@@ -743,12 +780,8 @@ static bool direct_ok(int kind, const void* p, int64_t ld, int64_t contiguous)
 }
 
 template <class T, bool ACOL, bool BCOL>
-static void launch_gemm(const Plan& p, bool direct, GemmArgs& g, hipStream_t stream)
+static void launch_gemm(const Plan& p, bool direct, const GemmArgs& g, hipStream_t stream)
 {
-    g.tiles_m = (int)((g.M + p.bm - 1) / p.bm);
-    g.tiles_n = (int)((g.N + p.bn - 1) / p.bn);
-    if (g.tiles_n == 0) g.tiles_n = 1;               // (column sums alone)
-    g.k_split = p.k_split;
     const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)p.splits);
 #define GEMM(BM, BN, WM, WN, DIRECT) \
     hipLaunchKernelGGL((gemm_kernel<T, ACOL, BCOL, BM, BN, WM, WN, DIRECT>), grid, dim3(WM * WN * 64), 0, stream, g)
@@ -777,47 +810,81 @@ static void launch_few_rows(const GemmArgs& g, hipStream_t stream)
     }
 }
 
-// layout 0: rows x rows, 1: rows x columns, 2: columns x columns
-template <class T>
-static int run_gemm(int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
+// One product, planned: layout 0: rows x rows, 1: rows x columns, 2: columns x columns.
+struct Job {
+    GemmArgs g;
+    Plan p;
+    bool direct;
+    int layout;
+};
+
+// Plans a product and takes what it needs of the workspace.
+static int plan_job(Job& j, int kind, int layout, void* colsum, char*& ws, size_t& left)
 {
-    const int kind = KindOf<T>::value;
-    if (layout == 0 && g.M <= kFewRows) {
-        launch_few_rows<T>(g, stream);
-        return check_launch();
-    }
-    const bool direct = direct_ok(kind, g.a, g.lda, layout == 2 ? g.M : g.K) && direct_ok(kind, g.b, g.ldb, layout ? g.N : g.K);
-    const Plan p = plan(kind, g.M, g.N, g.K, direct);
-    if ((double)((g.M + p.bm - 1) / p.bm) * (double)((g.N + p.bn - 1) / p.bn) > 2147483647.0) return SMLVM_ERR_UNSUPPORTED;
-    float* ws = static_cast<float*>(workspace);
-    size_t need = 0;
+    GemmArgs& g = j.g;
+    j.layout = layout;
+    j.direct = direct_ok(kind, g.a, g.lda, layout == 2 ? g.M : g.K) && direct_ok(kind, g.b, g.ldb, layout ? g.N : g.K);
+    j.p = plan(kind, g.M, g.N, g.K, j.direct);
+    if ((double)((g.M + j.p.bm - 1) / j.p.bm) * (double)((g.N + j.p.bn - 1) / j.p.bn) > 1.0e9) return SMLVM_ERR_UNSUPPORTED;
+    g.tiles_m = (int)((g.M + j.p.bm - 1) / j.p.bm);
+    g.tiles_n = (int)((g.N + j.p.bn - 1) / j.p.bn);
+    if (g.tiles_n == 0) g.tiles_n = 1;               // (column sums alone)
+    g.k_split = j.p.k_split;
     g.colsum = colsum;
-    if (p.splits > 1) {
-        g.part = ws;
-        need += (size_t)p.splits * g.M * g.N;
-        if (colsum) {
-            g.colsum_part = ws + need;
-            need += (size_t)p.splits * g.M;
+    if (j.p.splits > 1) {
+        const size_t part = (size_t)j.p.splits * g.M * g.N, sums = colsum ? (size_t)j.p.splits * g.M : 0;
+        const size_t need = (part + sums) * sizeof(float);
+        if (!ws || left < need) return SMLVM_ERR_WORKSPACE;
+        g.part = reinterpret_cast<float*>(ws);
+        if (colsum) g.colsum_part = g.part + part;
+        ws += need;
+        left -= need;
+    }
+    return SMLVM_OK;
+}
+
+static Join join_of(const Job& j)
+{
+    if (j.p.splits <= 1) return Join{0, 0, 0};
+    const int64_t want = (j.g.M * ((j.g.N + 7) / 8) + 255) / 256;
+    return Join{j.p.splits, (int)(want < 8192 ? want : 8192), j.g.colsum ? (int)((j.g.M + 255) / 256) : 0};
+}
+
+// one product, or a layer's dx and dw
+template <class T>
+static int launch_jobs(const Job* jobs, int count, hipStream_t stream)
+{
+    const Job& a = jobs[0];
+    const Job& b = jobs[count - 1];
+    if (count == 2 && a.p.bm == 64 && b.p.bm == 64) {
+        const int64_t blocks_a = (int64_t)a.g.tiles_m * a.g.tiles_n * a.p.splits, blocks_b = (int64_t)b.g.tiles_m * b.g.tiles_n * b.p.splits;
+        if (blocks_a + blocks_b > 0x7FFFFFFF) return SMLVM_ERR_UNSUPPORTED;
+        const dim3 grid((unsigned)(blocks_a + blocks_b));
+        if (sizeof(T) == 2 && a.direct && b.direct) {
+            if constexpr (sizeof(T) == 2)
+                hipLaunchKernelGGL((pair_kernel<T, true>), grid, dim3(256), 0, stream, a.g, b.g, (int)blocks_a);
+        } else {
+            hipLaunchKernelGGL((pair_kernel<T, false>), grid, dim3(256), 0, stream, a.g, b.g, (int)blocks_a);
+        }
+    } else {
+        for (int i = 0; i < count; ++i) {
+            const Job& j = jobs[i];
+            if (j.layout == 0) launch_gemm<T, false, false>(j.p, j.direct, j.g, stream);
+            else if (j.layout == 1) launch_gemm<T, false, true>(j.p, j.direct, j.g, stream);
+            else launch_gemm<T, true, true>(j.p, j.direct, j.g, stream);
         }
     }
-    if (need && (!ws || bytes < need * sizeof(float))) return SMLVM_ERR_WORKSPACE;
-    if (layout == 0) launch_gemm<T, false, false>(p, direct, g, stream);
-    else if (layout == 1) launch_gemm<T, false, true>(p, direct, g, stream);
-    else launch_gemm<T, true, true>(p, direct, g, stream);
-    if (p.splits > 1) {
-        const int64_t want = (g.M * ((g.N + 7) / 8) + 255) / 256;
-        const int blocks = (int)(want < 8192 ? want : 8192);
-        const int64_t sums = colsum ? (g.M + 255) / 256 : 0;
-        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + sums)), dim3(256), 0, stream, g, p.splits, blocks);
-    }
+    const Join ja = join_of(a), jb = count == 2 ? join_of(b) : Join{0, 0, 0};
+    const int64_t blocks = (int64_t)ja.blocks + ja.sum_blocks + jb.blocks + jb.sum_blocks;
+    if (blocks) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a.g, ja, b.g, jb);
     return check_launch();
 }
 
-static int dispatch_gemm(int kind, int layout, GemmArgs& g, void* colsum, void* workspace, size_t bytes, hipStream_t stream)
+static int launch_kind(int kind, const Job* jobs, int count, hipStream_t stream)
 {
-    if (kind == SMLVM_F32) return run_gemm<float>(layout, g, colsum, workspace, bytes, stream);
-    if (kind == SMLVM_F16) return run_gemm<f16_t>(layout, g, colsum, workspace, bytes, stream);
-    return run_gemm<bf16_t>(layout, g, colsum, workspace, bytes, stream);
+    if (kind == SMLVM_F32) return launch_jobs<float>(jobs, count, stream);
+    if (kind == SMLVM_F16) return launch_jobs<f16_t>(jobs, count, stream);
+    return launch_jobs<bf16_t>(jobs, count, stream);
 }
 
 static size_t workspace_of(int kind, int64_t M, int64_t N, int64_t K, bool colsum)
@@ -855,7 +922,7 @@ extern "C" size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, in
 {
     if (check_sizes(kind, M, N, K) != 1) return 0;
     const size_t dx = workspace_of(kind, M, K, N, false), dw = workspace_of(kind, N, K, M, true);
-    return (dx > dw ? dx : dw) + (act ? act_bytes(kind, M, N) : 0);
+    return dx + dw + (act ? act_bytes(kind, M, N) : 0);
 }
 
 extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -870,7 +937,16 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
     GemmArgs g = {};
     g.a = x; g.b = w; g.lda = ldx; g.ldb = ldw; g.M = M; g.N = N; g.K = K;
     g.out = y; g.bias = bias; g.res = residual; g.ldr = ldr; g.pre = pre; g.act = act;
-    return dispatch_gemm(kind, 0, g, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
+    if (M <= kFewRows) {
+        if (kind == SMLVM_F32) launch_few_rows<float>(g, (hipStream_t)stream);
+        else if (kind == SMLVM_F16) launch_few_rows<f16_t>(g, (hipStream_t)stream);
+        else launch_few_rows<bf16_t>(g, (hipStream_t)stream);
+        return check_launch();
+    }
+    Job job = {g, {}, false, 0};
+    char* ws = static_cast<char*>(workspace);
+    const int rc = plan_job(job, kind, 0, nullptr, ws, workspace_bytes);
+    return rc == SMLVM_OK ? launch_kind(kind, &job, 1, (hipStream_t)stream) : rc;
 }
 
 extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int32_t h_is_y, const void* x, int64_t ldx,
@@ -904,18 +980,20 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
         ws += bytes;
         workspace_bytes -= bytes;
     }
-    int rc = SMLVM_OK;
+    Job jobs[2];
+    int count = 0, rc = SMLVM_OK;
     if (dx && M && K) {
-        GemmArgs g = {};
-        g.a = dy; g.b = w; g.lda = ldy; g.ldb = ldw; g.M = M; g.N = K; g.K = N;
-        g.out = dx;
-        rc = dispatch_gemm(kind, 1, g, nullptr, ws, workspace_bytes, stream);
+        Job& j = jobs[count++];
+        j.g = GemmArgs{};
+        j.g.a = dy; j.g.b = w; j.g.lda = ldy; j.g.ldb = ldw; j.g.M = M; j.g.N = K; j.g.K = N; j.g.out = dx;
+        rc = plan_job(j, kind, 1, nullptr, ws, workspace_bytes);
     }
     if (rc == SMLVM_OK && N && (K ? dw != nullptr : db != nullptr)) {
-        GemmArgs g = {};
-        g.a = dy; g.b = x; g.lda = ldy; g.ldb = ldx; g.M = N; g.N = K; g.K = M;
-        g.out = dw;
-        rc = dispatch_gemm(kind, 2, g, db, ws, workspace_bytes, stream);
+        Job& j = jobs[count++];
+        j.g = GemmArgs{};
+        j.g.a = dy; j.g.b = x; j.g.lda = ldy; j.g.ldb = ldx; j.g.M = N; j.g.N = K; j.g.K = M; j.g.out = dw;
+        rc = plan_job(j, kind, 2, db, ws, workspace_bytes);
     }
-    return rc;
+    if (rc != SMLVM_OK || count == 0) return rc;
+    return launch_kind(kind, jobs, count, stream);
 }
