@@ -865,46 +865,49 @@ def token_logprobs_fwd(logits, actions, mask=None, want_stats=True):
 
 
 def token_logprobs_bwd(logits, actions, mask, stats, c, h, g=None, out=None):
-    """dlogits [B,T,V] = g (c dlogp + h dentropy); out: a buffer that holds the result for g = 1 already
-    (it is written only where g is another number)."""
+    """dlogits [B,T,V] = g (c dlogp + h dentropy); stats, c, h: tensors, or addresses of such; out: a buffer
+    that holds the result for g = 1 already (it is written only where g is another number)."""
     logits = _need_rows(logits)
     B, T, V = logits.shape
-    keep = out is not None
+    keep = 0 if out is None else 1
     if out is None:
         out = torch.empty((B, T, V), dtype=logits.dtype, device=logits.device)
+    stats, c, h = (t if t is None or isinstance(t, int) else t.data_ptr() for t in (stats, c, h))
     with _on(logits.device):
-        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), _ptr(stats), _ptr(c), _ptr(h),
-                                              _ptr(g), 1 if keep else 0, _ptr(out), B, T, V,
-                                              _stream_ptr()), "smlvm_token_logprobs_bwd")
+        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), stats, c, h, _ptr(g), keep, _ptr(out), B, T,
+                                              V, _stream_ptr()), "smlvm_token_logprobs_bwd")
     return out
+
+
+def policy_kept(kept):
+    """(stats, c, h) of `policy_loss`'s `kept` as addresses for token_logprobs_bwd."""
+    rows, at = kept.numel() // 5, kept.data_ptr()
+    return at, at + 12 * rows, at + 16 * rows
 
 
 def policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff, entropy_coeff,
                 mean, want_grad):
-    """-> dict(loss [1], logp, entropy, kl, clipped [B,T], stats [B,T,3], c, h [B,T], dlogits [B,T,V] or None)."""
+    """-> (loss [], logp, entropy, kl [B,T], clipped [B,T] bool, kept [5 B T], dlogits [B,T,V] or None); `kept` is what
+    the backward needs (policy_kept)."""
     logits = _need_rows(logits)
     B, T, V = logits.shape
     dev = logits.device
     rows = B * T
-    # two allocations for the fp32 outputs (64 rows of a small policy are launch bound): what the caller
-    # gets, and what the backward keeps
-    seen = torch.empty(rows * 3 + 1, dtype=torch.float32, device=dev)
-    kept = torch.empty(rows * 5, dtype=torch.float32, device=dev)
-    out = {k: seen[1 + i * rows:1 + (i + 1) * rows].view(B, T) for i, k in enumerate(("logp", "entropy", "kl"))}
-    out.update(loss=seen[:1], stats=kept[:3 * rows].view(B, T, 3), c=kept[3 * rows:4 * rows].view(B, T),
-               h=kept[4 * rows:].view(B, T))
-    out["clipped"] = torch.empty((B, T), dtype=torch.bool, device=dev)
-    out["dlogits"] = torch.empty((B, T, V), dtype=logits.dtype, device=dev) if want_grad else None
-    nbytes = lib().smlvm_policy_loss_workspace_bytes(rows)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    logp, entropy, kl = torch.empty((3, B, T), dtype=torch.float32, device=dev).unbind(0)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kept = torch.empty(rows * 5, dtype=torch.float32, device=dev)        # stats [rows, 3], c [rows], h [rows]
+    stats, c, h = policy_kept(kept)
+    clipped = torch.empty((B, T), dtype=torch.bool, device=dev)
+    dlogits = torch.empty((B, T, V), dtype=logits.dtype, device=dev) if want_grad else None
+    nbytes = 8 * (rows + 1)                                              # smlvm_policy_loss_workspace_bytes
+    ws = torch.empty(rows + 1, dtype=torch.float64, device=dev)
     with _on(dev):
         _check(lib().smlvm_policy_loss(
-            *_rows_args(logits, actions, mask), _ptr(old_logp), _ptr(advantages), _ptr(ref_logp), clip_low,
-            clip_high, kl_coeff, entropy_coeff, 1 if mean else 0, _ptr(out["loss"]),
-            _ptr(out["logp"]), _ptr(out["entropy"]), _ptr(out["kl"]), _ptr(out["clipped"]), _ptr(out["stats"]), _ptr(out["c"]),
-            _ptr(out["h"]), _ptr(out["dlogits"]), B, T, V, _ptr(ws), nbytes, _stream_ptr()),
+            *_rows_args(logits, actions, mask), _ptr(old_logp), _ptr(advantages), _ptr(ref_logp), clip_low, clip_high,
+            kl_coeff, entropy_coeff, 1 if mean else 0, loss.data_ptr(), logp.data_ptr(), entropy.data_ptr(), kl.data_ptr(),
+            clipped.data_ptr(), stats, c, h, _ptr(dlogits), B, T, V, ws.data_ptr(), nbytes, _stream_ptr()),
             "smlvm_policy_loss")
-    return out
+    return loss, logp, entropy, kl, clipped, kept, dlogits
 
 
 def capture_id():

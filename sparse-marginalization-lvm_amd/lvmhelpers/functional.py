@@ -362,27 +362,26 @@ class _ClippedPolicyLoss(torch.autograd.Function):
                 entropy_coeff, mean):
         want = ctx.needs_input_grad[0]
         ctx.set_materialize_grads(False)      # (no zeros for the statistics' gradients)
-        out = _native.policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff,
-                                  entropy_coeff, mean, want)
+        loss, logp, entropy, kl, clipped, kept, dlogits = _native.policy_loss(
+            logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff, entropy_coeff, mean, want)
         if want:
             ctx.has_mask = mask is not None
-            ctx.save_for_backward(logits, actions, out["stats"], out["c"], out["h"],
-                                  *([mask] if mask is not None else []))
-            ctx.ready = out["dlogits"]
+            ctx.save_for_backward(logits, actions, kept, *([mask] if mask is not None else []))
+            ctx.ready = dlogits
             ctx.capture = _native.capture_id()
-        ctx.mark_non_differentiable(out["logp"], out["entropy"], out["kl"], out["clipped"])
-        return out["loss"].reshape(()), out["logp"], out["entropy"], out["kl"], out["clipped"]
+        ctx.mark_non_differentiable(logp, entropy, kl, clipped)
+        return loss, logp, entropy, kl, clipped
 
     @staticmethod
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 11
-        logits, actions, stats, c, h = ctx.saved_tensors[:5]
-        mask = ctx.saved_tensors[5] if ctx.has_mask else None
+        logits, actions, kept = ctx.saved_tensors[:3]
+        mask = ctx.saved_tensors[3] if ctx.has_mask else None
         ready, ctx.ready = ctx.ready, None
         if ready is not None and _native.capture_id() != ctx.capture:
             ready = None
-        dlogits = _native.token_logprobs_bwd(logits, actions, mask, stats, c, h,
+        dlogits = _native.token_logprobs_bwd(logits, actions, mask, *_native.policy_kept(kept),
                                              g=g.to(torch.float32).contiguous(), out=ready)
         return (dlogits,) + (None,) * 10
 
@@ -410,7 +409,10 @@ def _row_values(t, lead, logits, name, what, dtype):
         raise ValueError(f"{name}: {what} is a constant of the loss; detach it (no gradient would reach it)")
     if t.dtype != dtype:
         t = t.to(dtype)
-    return t.detach().reshape(logits.shape[:2]).contiguous()
+    if t.requires_grad:          # (gradients are off)
+        t = t.detach()
+    shape = logits.shape[:2]
+    return (t if t.shape == shape else t.reshape(shape)).contiguous()
 
 
 def _row_mask(mask, lead, logits, name):
@@ -472,7 +474,8 @@ def clipped_policy_loss(logits, actions, old_logp, advantages, ref_logp=None, ma
     loss, logp, entropy, kl, clipped = _ClippedPolicyLoss.apply(
         rows, act, old, adv, ref, _row_mask(mask, lead, rows, name), float(clip_low), float(clip_high),
         float(kl_coeff), float(entropy_coeff), reduction == "mean")
-    return loss, {"logp": logp.view(lead), "entropy": entropy.view(lead), "kl": kl.view(lead), "clipped": clipped.view(lead)}
+    stats = {"logp": logp, "entropy": entropy, "kl": kl, "clipped": clipped}
+    return loss, stats if len(lead) == 2 else {k: v.view(lead) for k, v in stats.items()}
 
 
 _NARROW = (torch.float16, torch.bfloat16)
