@@ -338,6 +338,37 @@ def test_state_dict_round_trip_keeps_types_and_addresses(dev, bits):
     assert torch.equal(q, after) and other.state[q]["exp_avg"].dtype == opt.state[p]["exp_avg"].dtype
 
 
+def test_replaced_weights_and_states_are_seen(dev):
+    """A weight whose storage, and a state whose tensors were exchanged between two steps (weights moved, states
+    restored by hand); a parameter resized behind the optimiser's back is refused."""
+    p = torch.nn.Parameter(_param((64, 64), torch.float32, dev, 1))
+    opt = _optim().AdamW([p], lr=1e-2, weight_decay=0.05)
+    ref = Reference(p, 32, 0)
+    for t in range(4):
+        p.grad = _grad((64, 64), torch.float32, dev, t)
+        opt.step()
+        ref.step(_flat(p.grad), torch.float32).check(p, opt.state[p])
+        if t == 1:
+            p.data = p.data.clone()
+        if t == 2:
+            opt.state[p] = {k: v.clone() for k, v in opt.state[p].items()}
+    on_gpu = p.data
+    p.data = on_gpu.cpu()                       # (the state stays behind; the gradient goes with it)
+    p.grad = torch.zeros(64, 64)
+    with pytest.raises(RuntimeError):
+        opt.step()
+    p.grad = None
+    p.data = torch.zeros(64, 65, device=dev)
+    p.grad = torch.zeros(64, 65, device=dev)
+    with pytest.raises(ValueError):
+        opt.step()
+    q = torch.nn.Parameter(torch.zeros(10, 4, device=dev))
+    opt = _optim().AdamW([q])
+    q.grad = torch.sparse_coo_tensor(torch.tensor([[1]], device=dev), torch.ones(1, 4, device=dev), (10, 4))
+    with pytest.raises(TypeError):
+        opt.step()
+
+
 def test_small_parameters_keep_32_bits(dev):
     w, b = _param((64, 64), torch.float32, dev, 1), _param((64,), torch.float32, dev, 2)
     opt = _optim().AdamW([w, b], state_bits=8)
