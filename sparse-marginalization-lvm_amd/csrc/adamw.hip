@@ -57,21 +57,58 @@ __device__ __forceinline__ int scale_exponent(float top)
 }
 __device__ __forceinline__ float pow2f(int k) { return __builtin_bit_cast(float, (uint32_t)(k + 127) << 23); }
 
+// Square roots of 8 values >= 0, correctly rounded (but for what lies within 2^-46 of a midpoint) in 5
+// instructions each: the residual of v rsq(v) is exact in an fma, and half of rsq(v) times it is the correction.
+// A wave that holds a zero, a subnormal number, an infinity or a NaN takes sqrtf.
+__device__ __forceinline__ void sqrt8(float (&v)[8])
+{
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) odd |= __builtin_amdgcn_classf(v[j], 0x2F3);
+    if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = sqrtf(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float r = __builtin_amdgcn_rsqf(v[j]);
+            const float s = v[j] * r;
+            v[j] = fmaf(fmaf(-s, s, v[j]), 0.5f * r, s);
+        }
+    }
+}
+
 // e4m3 code of x * 2^-k, rounded up with probability u16 / 2^16 of the distance (FLOOR: positive values
-// keep at least the smallest code).  Scaling by powers of two is exact, |y| / q < 16 has 20 fraction
-// bits in fp32 and u16 / 2^16 has 16, so the sum's whole part is exact.
+// keep at least the smallest code).  From 2^-6 on a code is the top of the fp32 pattern: 20 mantissa bits lie
+// below it, the random ones are added to the upper 16 of those and the sum cut off, carries into the
+// exponent included.  Below, codes are 2^-9 apart.
 template <bool FLOOR>
 __device__ __forceinline__ uint32_t encode_e4m3(float x, float inv_scale, uint32_t u16)
 {
     const float y = fabsf(x) * inv_scale;
-    int e = (int)(__builtin_bit_cast(uint32_t, y) >> 23) - 127;
-    e = e < -6 ? -6 : e;
-    const float s = fmaf((float)u16, 0x1p-16f, y * pow2f(3 - e));
-    int code = (e + 6) * 8 + (int)s;                            // (int)s in [8, 16] from the exponent -6 on
-    code = code > 0x7E ? 0x7E : code;
-    if constexpr (FLOOR) code = (code == 0 && y > 0.0f) ? 1 : code;
+    const uint32_t raw = ((__builtin_bit_cast(uint32_t, y) + (u16 << 4)) >> 20) - (120u << 3);
+    const uint32_t low = (uint32_t)fmaf(y, 512.0f, (float)u16 * 0x1p-16f);
+    uint32_t code = y < 0x1p-6f ? low : raw > 0x7Eu ? 0x7Eu : raw;
+    if constexpr (FLOOR) code = code == 0 && y > 0.0f ? 1u : code;
     if (!finite_f32(x)) code = 0x7F;
-    return (uint32_t)code | (FLOOR ? 0u : (__builtin_bit_cast(uint32_t, x) >> 24) & 0x80u);
+    return code | (FLOOR ? 0u : (__builtin_bit_cast(uint32_t, x) >> 24) & 0x80u);
+}
+
+// Largest finite |x| of 8 values in each of 32 lanes: fmaxf passes NaN over, infinities are sorted out where
+// there are any.
+__device__ __forceinline__ float block_top(const float (&x)[8])
+{
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+    top = group_reduce<32>(top, OpMaxF{});
+    if (__builtin_amdgcn_ballot_w64(!finite_f32(top)) != 0) {     // (uniform: the whole wave takes it)
+        float t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t = finite_f32(x[j]) ? fmaxf(t, fabsf(x[j])) : t;
+        top = group_reduce<32>(t, OpMaxF{});
+    }
+    return top;
 }
 
 __device__ __forceinline__ void decode_e4m3(u32x2 codes, float scale, float (&x)[8])
@@ -166,8 +203,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamwTable table,
             }
             if (whole) { store_vec(m_, m); store_vec(v_, v); }
             else { store_some(m_, have, m); store_some(v_, have, v); }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = sqrtf(v[j]);
+            sqrt8(v);
         } else {
             uint8_t* const m_ = static_cast<uint8_t*>(t.m) + at;
             uint8_t* const r_ = static_cast<uint8_t*>(t.v) + at;
@@ -175,20 +211,16 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamwTable table,
             const float ms = have ? t.m_scale[block] : 0.0f, rs = have ? t.r_scale[block] : 0.0f;
             decode_e4m3(load_codes(m_, have, whole), ms, m);
             decode_e4m3(load_codes(r_, have, whole), rs, v);
-            float mtop = 0.0f, rtop = 0.0f;
             // fp64 averages, rounded once: which code and which scale a value gets then does not depend
             // on how its sum was associated
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const double gd = (double)g[j], rd = (double)v[j];
                 m[j] = (float)fma(hp.beta1, (double)m[j], (1.0 - hp.beta1) * gd);
-                v[j] = sqrtf((float)fma(hp.beta2, rd * rd, (1.0 - hp.beta2) * (gd * gd)));
-                if (finite_f32(m[j])) mtop = fmaxf(mtop, fabsf(m[j]));
-                if (finite_f32(v[j])) rtop = fmaxf(rtop, v[j]);
+                v[j] = (float)fma(hp.beta2, rd * rd, (1.0 - hp.beta2) * (gd * gd));
             }
-            mtop = group_reduce<32>(mtop, OpMaxF{});
-            rtop = group_reduce<32>(rtop, OpMaxF{});
-            const int mk = scale_exponent(mtop), rk = scale_exponent(rtop);
+            sqrt8(v);
+            const int mk = scale_exponent(block_top(m)), rk = scale_exponent(block_top(v));
             const float minv = pow2f(-mk), rinv = pow2f(-rk);
             u32x2 mc = {0u, 0u}, rc = {0u, 0u};
             const uint32_t key = key0 + (uint32_t)((uint64_t)at >> 32);
@@ -207,7 +239,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamwTable table,
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)                              // v holds sqrt(v) here
-            p[j] = fmaf(-step_size, m[j] / fmaf(v[j], rsqrt2, hp.eps), p[j] * keep);
+            // (the hardware's reciprocal, 1 ulp, for a division of ten instructions)
+            p[j] = fmaf(-step_size, m[j] * __builtin_amdgcn_rcpf(fmaf(v[j], rsqrt2, hp.eps)), p[j] * keep);
         if (whole) store_vec(p_ + at, p); else store_some(p_ + at, have, p);
     }
 
