@@ -390,7 +390,7 @@ static void launch_rows(const RowsIn& in, const RowsOut& out, const Policy& pol,
     else if (nv <= 2048) ROWS(256, 8);
     else if (nv <= 4096) ROWS(512, 8);
     else if (nv <= 8192) ROWS(512, 16);
-    else if (nv <= 16384) ROWS(1024, 16);
+    else if (nv <= 16384) ROWS(512, 32);
     else ROWS(1024, 0);
 #undef ROWS
 }

@@ -86,7 +86,7 @@ class Reference:
             self.m = (b1 * m0 + (1 - b1) * g).float().double()
             self.v = (b2 * r0 * r0 + (1 - b2) * g * g).float().double()
             u = _random(self.p.numel(), self.seed, self.t, self.index)
-            r = self.v.float().sqrt().double()
+            r = self.v.sqrt().float().double()      # (fp32's own root may come from a vector library that rounds otherwise)
             for i, (x, bits, floor) in enumerate(((self.m, u & 0xFFFF, False), (r, u >> 16, True))):
                 self.codes[i], self.scales[i] = _encode(x, bits, floor)
             self.mtol = U * self.m.abs()
@@ -174,6 +174,18 @@ def test_any_dense_memory_order_and_alignment(dev, bits):
             in_order = g.permute(o).contiguous().reshape(-1)
             r.step(in_order, torch.float32).check(p, opt.state[p])
     assert torch.equal(flat[:3], before[:3]) and torch.equal(flat[4999:], before[4999:])
+
+
+@pytest.mark.parametrize("bits,n", [(32, 8_500_001), (8, 16_900_003)])
+def test_a_large_tensor_counts_once(dev, bits, n):
+    """Over 4096 workgroups (the step is counted by a launch of its own), several passes per workgroup (8 bits)."""
+    p = _param((n,), torch.float32, dev, 1)
+    opt = _optim().AdamW([p], lr=1e-2, weight_decay=0.05, state_bits=bits, min_8bit_size=1)
+    ref = Reference(p, bits, 0)
+    for t in range(2):
+        g = _grad((n,), torch.float32, dev, t)
+        opt.step(grads=[g])
+        ref.step(g, torch.float32).check(p, opt.state[p])
 
 
 def test_more_tensors_than_one_launch_holds_and_missing_gradients(dev):
