@@ -312,34 +312,39 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(const RowsIn in
     }
 }
 
-// The backward from saved statistics: blockIdx.y splits long rows.
+// The backward from saved statistics.  Workgroups go over (row or group of rows, part of a long row) units; a
+// bounded number of them, so that the call that has nothing to write (keep_if_one) is over at once (65536
+// workgroups took 16 us to find out).
 template <class T, int G>
 __global__ __launch_bounds__(256) void rows_bwd_kernel(const RowsIn in, const float* __restrict__ stats,
                                                        const float* __restrict__ c_, const float* __restrict__ h_,
                                                        const float* __restrict__ g_, int keep_if_one,
-                                                       T* __restrict__ out)
+                                                       T* __restrict__ out, uint32_t units, uint32_t parts)
 {
     constexpr int P = kPer<T>;
     const float g = g_ ? *g_ : 1.0f;
     if (keep_if_one && g == 1.0f) return;
-    const uint32_t row = blockIdx.x * (256 / G) + threadIdx.x / G;
-    if (row >= in.rows) return;
     const int lane = threadIdx.x & (G - 1);
-    T* const dz = out + (int64_t)row * in.V;
-    const int64_t first = (int64_t)blockIdx.y * G + lane, step = (int64_t)gridDim.y * G;
-    if (in.mask && in.mask[row] == 0) {
-        float zero[P] = {};
-        for (int64_t v = first; v * P < in.V; v += step) store_row_vec<T>(dz, (int)v, in.V, zero);
-        return;
+    for (uint32_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const uint32_t row = (unit / parts) * (256 / G) + threadIdx.x / G, part = unit % parts;
+        if (row >= in.rows) continue;
+        T* const dz = out + (int64_t)row * in.V;
+        const int64_t first = (int64_t)part * G + lane, step = (int64_t)parts * G;
+        if (in.mask && in.mask[row] == 0) {
+            float zero[P] = {};
+            for (int64_t v = first; v * P < in.V; v += step) store_row_vec<T>(dz, (int)v, in.V, zero);
+            continue;
+        }
+        const T* const z = row_of<T>(in, row);
+        const float m = stats[3 * (int64_t)row], s = stats[3 * (int64_t)row + 1], ent = stats[3 * (int64_t)row + 2];
+        const float inv = 1.0f / s;
+        const float c = g * c_[row], h = h_ ? g * h_[row] : 0.0f;
+        const float ln2 = (float)kLn2d;
+        const Slope sl = {h_ ? (c + h * (ent - ln2 * log2f(s))) * inv : c * inv, h * ln2 * inv, c};
+        const int64_t action = in.actions[row];
+        for (int64_t v = first; v * P < in.V; v += step)
+            gradient_vec<T>(load_row_vec<T>(z, (int)v, in.V), dz, (int)v, in.V, m, sl, action);
     }
-    const T* const z = row_of<T>(in, row);
-    const float m = stats[3 * (int64_t)row], s = stats[3 * (int64_t)row + 1], ent = stats[3 * (int64_t)row + 2];
-    const float inv = 1.0f / s;
-    const float c = g * c_[row], h = h_ ? g * h_[row] : 0.0f;
-    const float ln2 = (float)kLn2d;
-    const Slope sl = {h_ ? (c + h * (ent - ln2 * log2f(s))) * inv : c * inv, h * ln2 * inv, c};
-    for (int64_t v = first; v * P < in.V; v += step)
-        gradient_vec<T>(load_row_vec<T>(z, (int)v, in.V), dz, (int)v, in.V, m, sl, in.actions[row]);
 }
 
 // norm = 1 / max(1, number of rows that count)
@@ -400,17 +405,23 @@ static void launch_bwd(const RowsIn& in, const float* stats, const float* c, con
                        int keep, void* dz, hipStream_t stream)
 {
     const int64_t nv = ((int64_t)in.V + kPer<T> - 1) / kPer<T>;
-    if (nv <= 8) {
-        hipLaunchKernelGGL((rows_bwd_kernel<T, 8>), dim3((in.rows + 31) / 32), dim3(256), 0, stream, in, stats, c,
-                           h, g, keep, static_cast<T*>(dz));
-    } else if (nv <= 128) {
-        hipLaunchKernelGGL((rows_bwd_kernel<T, 64>), dim3((in.rows + 3) / 4), dim3(256), 0, stream, in, stats, c,
-                           h, g, keep, static_cast<T*>(dz));
-    } else {
-        const int64_t split = (nv + 256 * 8 - 1) / (256 * 8);      // some 8 vectors per thread
-        hipLaunchKernelGGL((rows_bwd_kernel<T, 256>), dim3(in.rows, (unsigned)(split < 64 ? split : 64)), dim3(256), 0,
-                           stream, in, stats, c, h, g, keep, static_cast<T*>(dz));
+    const int group = nv <= 8 ? 8 : nv <= 128 ? 64 : 256;
+    const int64_t row_units = ((int64_t)in.rows * group + 255) / 256;
+    int64_t parts = 1;                                   // few long rows: parts of at least 4 vectors per thread
+    if (group == 256 && row_units < 2048) {
+        parts = (2048 + row_units - 1) / row_units;
+        const int64_t most = (nv + 1023) / 1024;
+        if (parts > most) parts = most;
     }
+    const int64_t units = row_units * parts;
+    const dim3 grid((unsigned)(units < 4096 ? units : 4096));
+#define ROWS_BWD(G)                                                                                              \
+    hipLaunchKernelGGL((rows_bwd_kernel<T, G>), grid, dim3(256), 0, stream, in, stats, c, h, g, keep,            \
+                       static_cast<T*>(dz), (uint32_t)units, (uint32_t)parts)
+    if (group == 8) ROWS_BWD(8);
+    else if (group == 64) ROWS_BWD(64);
+    else ROWS_BWD(256);
+#undef ROWS_BWD
 }
 
 // 0: nothing to do, 1: go on, negative: an error
