@@ -192,8 +192,10 @@ __device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n,
 
 // ------------------------------------------------------------------------------------- staging
 // A tile of ROWS m (n) by BK k.  Row operand in LDS: [ROWS][BK] 16-bit elements, the 16-byte slots of a row
-// exchanged by slot ^ f(row) so that 16 lanes reading one slot of 16 rows touch every bank once;
-// column operand: [BK][ROWS], the 32-byte chunks of a k row exchanged by chunk ^ (k & 7).
+// exchanged by slot ^ f(row); column operand: [BK][ROWS], the 32-byte chunks of a k row exchanged by
+// chunk ^ f(k).  The fs put the addresses that one LDS cycle serves on different banks: for 16-byte reads lanes 0-3,
+// 12-15, 20-27 (and the like), for the transposing 8-byte ones 32 neighbours, that is k rows 0-3 and 8-11.
+// (With f = row / 4 and f = k & 7 a fifth of the LDS cycles of dw's kernel were conflicts.)
 template <int ROWS, int BK, bool COL>
 struct Tile {
     static constexpr int kBytes = ROWS * BK * 2;
@@ -202,25 +204,36 @@ struct Tile {
     static constexpr int kMask = COL ? (ROWS / 16 < 8 ? ROWS / 16 : 8) - 1 : kPerRow - 1;
     static_assert(BK == 32 || BK == 64, "swizzles below");
 
+    __device__ __forceinline__ static int swizzle(int row)
+    {
+        if constexpr (COL) {
+            return kMask == 7 ? (row & 3) | ((row >> 1) & 4) : ((row >> 1) & 1) | ((row >> 2) & 2);
+        } else if constexpr (kPerRow == 8) {
+            return (row >> 1) & 7;
+        } else {
+            const int r = (row >> 2) & 3;
+            return (((r ^ (r >> 1)) & 1) << 1) | (r >> 1);
+        }
+    }
     // 16-byte slot -> (stored row, first element in it) of the source
     __device__ __forceinline__ static void source(int slot, int& row, int& at)
     {
         row = slot / kPerRow;
         const int s = slot % kPerRow;
-        if constexpr (COL) at = (((s >> 1) ^ (row & kMask)) << 4) + ((s & 1) << 3);
-        else at = (s ^ ((row / (16 / kPerRow)) & kMask)) << 3;
+        if constexpr (COL) at = (((s >> 1) ^ swizzle(row)) << 4) + ((s & 1) << 3);
+        else at = (s ^ swizzle(row)) << 3;
     }
     // lane's 8 k of row `base + lane % 16`, k step kk (of 32): byte offset (row operand)
     __device__ __forceinline__ static int row_at(int base, int kk, int lane)
     {
         const int row = base + (lane & 15), s = kk * 4 + (lane >> 4);
-        return row * (BK * 2) + ((s ^ ((row / (16 / kPerRow)) & kMask)) << 4);
+        return row * (BK * 2) + ((s ^ swizzle(row)) << 4);
     }
     // column operand: p-th (of two) transposing reads
     __device__ __forceinline__ static int col_at(int base, int kk, int p, int lane)
     {
         const int k = kk * 32 + ((lane >> 4) << 3) + p * 4 + ((lane & 15) >> 2);
-        return k * (ROWS * 2) + (((base >> 4) ^ (k & kMask)) << 5) + ((lane & 3) << 3);
+        return k * (ROWS * 2) + (((base >> 4) ^ swizzle(k)) << 5) + ((lane & 3) << 3);
     }
     __device__ __forceinline__ static s16x8 fragment(const char* tile, int base, int kk, int lane)
     {
