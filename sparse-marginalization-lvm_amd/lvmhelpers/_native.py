@@ -787,6 +787,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4, "tanh":
 
 def _rows(t, width):
     """A matrix whose rows are consecutive elements (any distance apart) -> (tensor, row stride)."""
+    if t.is_contiguous():
+        return t, width
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < width:
         t = t.contiguous()
     return t, max(t.stride(0), width)
@@ -801,13 +803,15 @@ def linear_fwd(x, w, bias, residual, act, want_pre):
     ldr = N
     if residual is not None:
         residual, ldr = _rows(residual, N)
-    kind = KINDS[x.dtype]
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    pre = torch.empty((M, N), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device) if want_pre else None
-    nbytes = lib().smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    with _on(x.device):
-        _check(lib().smlvm_linear_fwd(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, _ptr(y), _ptr(pre),
+    dt, dev = x.dtype, x.device
+    kind = KINDS[dt]
+    y = torch.empty((M, N), dtype=dt, device=dev)
+    pre = torch.empty((M, N), dtype=dt if dt == torch.float32 else torch.float16, device=dev) if want_pre else None
+    L = lib()
+    nbytes = L.smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev):
+        _check(L.smlvm_linear_fwd(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, _ptr(y), _ptr(pre),
                                       kind, act, M, N, K, _ptr(ws),
                                       nbytes, _stream_ptr()), "smlvm_linear_fwd")
     return y, pre

@@ -306,10 +306,11 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         raise ValueError(f"{name}: residual must be {tuple(out_shape)}, got {tuple(residual.shape)}")
     if not x.is_cuda:
         raise _native.NativeError(f"{name}: expected GPU tensors (the hot path has no CPU fallback)")
-    if x.dtype not in _native.KINDS:
-        raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {x.dtype}")
+    dtype, at = x.dtype, x.get_device()
+    if dtype not in _native.KINDS:
+        raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {dtype}")
     for t, what in ((weight, "weight"), (bias, "bias"), (residual, "residual")):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.dtype != dtype or t.get_device() != at):       # (-1 on the CPU)
             raise TypeError(f"{name}: {what} must have x's type and device ({x.dtype}, {x.device}), got {t.dtype}, {t.device}")
     if x.dim() != 2:
         x = x.reshape(-1, weight.shape[1]) if x.numel() else x.reshape(out_shape[:-1].numel(), weight.shape[1])
