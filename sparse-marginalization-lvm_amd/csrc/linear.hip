@@ -321,10 +321,11 @@ struct Through {
     static_assert(Tl::kSlots % THREADS == 0, "whole slots per thread");
     u32x4 held[kEach][kVecs];
     const T* from[kEach];                                               // the slot's elements at the current k
-    int64_t step;
+    int64_t ld, step;
 
-    __device__ __forceinline__ void init(const T* src, int64_t ld, int64_t first, int64_t k0)
+    __device__ __forceinline__ void init(const T* src, int64_t ld_, int64_t first, int64_t k0)
     {
+        ld = ld_;
         step = COL ? BK * ld : BK;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -334,9 +335,9 @@ struct Through {
         }
     }
     // `rows`: what is left of the matrix' m (n), `k_left` of this part's k, `k_all` of the matrix'; then on to the
-    // next k tile.  At an edge a slot that ends behind its row is read whole where another stored row
+    // next k tile.  At an edge a slot that ends behind its row is read whole where that much of the matrix
     // follows (the elements too many are of an m nobody stores, or a k that is cleared here), element by
-    // element in the last one.
+    // element at its end.
     __device__ __forceinline__ void load(int64_t rows, int64_t k_left, int64_t k_all)
     {
         if (rows >= ROWS && k_left >= BK) {                             // (uniform)
@@ -350,12 +351,13 @@ struct Through {
         }
         const int r_end = (int)(COL ? (k_left < BK ? k_left : BK) : (rows < ROWS ? rows : ROWS));
         const int c_end = (int)(COL ? (rows < ROWS ? rows : ROWS) : (k_left < BK ? k_left : BK));
-        const int64_t r_all = COL ? k_all : rows;
+        const int64_t r_all = COL ? k_all : rows, c_all = COL ? rows : k_all;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             int row, at;
             Tl::source(i * THREADS + threadIdx.x, row, at);
-            const bool in = row < r_end && at < c_end, whole = at + 8 <= c_end || row + 1 < r_all;
+            const bool in = row < r_end && at < c_end;
+            const bool whole = at + 8 <= c_end || at + 8 <= (r_all - 1 - row) * ld + c_all;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v) held[i][v] = u32x4{0u, 0u, 0u, 0u};
             if (in && whole) {

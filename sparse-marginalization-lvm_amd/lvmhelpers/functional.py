@@ -1,7 +1,17 @@
 """torch.autograd glue over the C-ABI kernels (``_native``).  Host-side plumbing only."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
+
+
+def _once(backward):
+    """once_differentiable for a backward, at no cost (3 us) where no graph of the backward is wanted."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _patterns_written(x, p, mask):
@@ -275,6 +285,7 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, dy):
         dx = dw = db = None
         want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
@@ -340,6 +351,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy
 
     @staticmethod
+    @_once
     def backward(ctx, glogp, gentropy):
         logits, actions, stats = ctx.saved_tensors[:3]
         mask = ctx.saved_tensors[3] if ctx.has_mask else None
@@ -374,6 +386,7 @@ class _ClippedPolicyLoss(torch.autograd.Function):
         return loss, logp, entropy, kl, clipped
 
     @staticmethod
+    @_once
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 11
@@ -409,6 +422,8 @@ def _row_values(t, lead, logits, name, what, dtype):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: {what} is a constant of the loss; detach it (no gradient would reach it)")
     if t.dtype != dtype:
+        if dtype == torch.float32 and t.dtype not in _NARROW:
+            raise TypeError(f"{name}: {what} must be float32, float16 or bfloat16, got {t.dtype}")
         t = t.to(dtype)
     if t.requires_grad:          # (gradients are off)
         t = t.detach()

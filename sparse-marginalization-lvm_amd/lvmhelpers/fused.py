@@ -54,13 +54,17 @@ def fuse_linears(module):
     """Replaces, in place, every nn.Linear inside the nn.Sequentials of `module` (itself included) by a
     LinearAct with the same parameters, taking the activation module that follows it into the
     epilogue; that one's place holds an nn.Identity, so that state_dict keys do not change.  Linears with
-    hooks, subclasses of nn.Linear and activations without an epilogue stay as they are.  Returns `module`."""
-    for seq in [m for m in module.modules() if isinstance(m, torch.nn.Sequential)]:
+    hooks or of another type than float32, float16, bfloat16, subclasses of nn.Linear and of nn.Sequential, and
+    activations without an epilogue stay as they are.  Returns `module`."""
+    def hooked(m):
+        return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+    for seq in [m for m in module.modules() if type(m) is torch.nn.Sequential]:
         for i, lin in enumerate(seq):
-            if type(lin) is not torch.nn.Linear or lin._forward_hooks or lin._forward_pre_hooks:
+            if type(lin) is not torch.nn.Linear or hooked(lin) or lin.weight.dtype not in _native.KINDS:
                 continue
             follow = seq[i + 1] if i + 1 < len(seq) else None
-            name = None if follow is None or follow._forward_hooks or follow._forward_pre_hooks else _activation_name(follow)
+            name = None if follow is None or hooked(follow) else _activation_name(follow)
             new = LinearAct.__new__(LinearAct)
             torch.nn.Module.__init__(new)
             new.in_features, new.out_features, new.activation = lin.in_features, lin.out_features, name or "none"

@@ -86,6 +86,9 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------------------------- state
     def _init_state(self, p, group):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a parameter's first step makes its state, which every replay of this capture would "
+                               "make anew; run one step before capturing (GraphedStep does)")
         if torch.empty_like(p).stride() != p.stride():
             raise ValueError("AdamW: a parameter's memory must be dense (no gaps, no overlap)")
         st = {"step": torch.zeros((), dtype=torch.int64, device=p.device)}

@@ -207,6 +207,54 @@ def test_neighbouring_memory_is_left_alone(dev):
             _within(y, base.double().cpu(), 4 * _half(dtype) * base.double().cpu().abs() + 1e-5)
 
 
+def test_more_than_2_to_the_31_elements(dev):
+    """x and dx of 70000 x 32768 bf16: rows and gradients far behind the first 2^31 elements."""
+    M, N, K = 70000, 16, 32768
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=dev)
+    for i in range(0, M, 10000):
+        x[i:i + 10000] = torch.randn(min(10000, M - i), K, device=dev, generator=torch.Generator(dev).manual_seed(i))
+    w = (torch.randn(N, K, generator=torch.Generator().manual_seed(1)) / 181).bfloat16().to(dev)
+    dy = torch.randn(M, N, generator=torch.Generator().manual_seed(2)).bfloat16().to(dev)
+    xl, wl = x.requires_grad_(True), w.requires_grad_(True)
+    y = _F().linear_act(xl, wl)
+    dx, dw = torch.autograd.grad(y, [xl, wl], dy)
+    rows = torch.tensor([0, 1, 65535, 65536, 65537, M - 2, M - 1], device=dev)
+    xs, ws, ds = x.detach()[rows].double(), w.detach().double(), dy[rows].double()
+    want = xs @ ws.t().contiguous()
+    _within(y.detach()[rows], want.cpu(), (_sum_err(K, torch.bfloat16) * (xs.abs() @ ws.abs().t().contiguous()) + 2.0 ** -8 * want.abs()).cpu())
+    want = ds @ ws
+    _within(dx[rows], want.cpu(), (_sum_err(N, torch.bfloat16) * (ds.abs() @ ws.abs()) + 2.0 ** -8 * want.abs()).cpu())
+    want = mag = 0.0
+    for i in range(0, M, 10000):
+        a, b = dy[i:i + 10000].double().t().contiguous(), x.detach()[i:i + 10000].double()
+        want, mag = want + a @ b, mag + a.abs() @ b.abs()
+    _within(dw, want.cpu(), (_sum_err(M, torch.bfloat16) * mag + 2.0 ** -8 * want.abs()).cpu())
+
+
+def test_tiny_matrices_at_the_end_of_their_memory(dev):
+    """Widths below one vector: what is read behind a row must still be the tensor's (the values there are NaN)."""
+    for dtype in FLOATS:
+        for M, N, K in ((5, 3, 1), (9, 2, 3), (70, 5, 7), (6, 70, 2)):
+            x, w, b, _, dy = _case(M, N, K, dtype, 4)
+            xb = torch.full((M * K + 64,), float("nan"), dtype=dtype, device=dev)
+            xb[:M * K] = x.reshape(-1).to(dev)
+            wb = torch.full((N * K + 64,), float("nan"), dtype=dtype, device=dev)
+            wb[:N * K] = w.reshape(-1).to(dev)
+            _check(dev, xb[:M * K].view(M, K).cpu(), wb[:N * K].view(N, K).cpu(), b, None, dy, "silu", dtype)
+            xv, wv = xb[:M * K].view(M, K).requires_grad_(True), wb[:N * K].view(N, K).requires_grad_(True)
+            y = _F().linear_act(xv, wv, b.to(dev), "silu")
+            grads = torch.autograd.grad(y, [xv, wv], dy.to(dev))
+            assert all(bool(t.isfinite().all()) for t in (y, *grads))
+
+
+def test_no_second_derivative(dev):
+    x = torch.randn(3, 4, device=dev, requires_grad=True)
+    w = torch.randn(5, 4, device=dev, requires_grad=True)
+    (dx,) = torch.autograd.grad(_F().linear_act(x, w, None, "silu").sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_captured_streams_and_repeats(dev, dtype):
     from lvmhelpers import graphs

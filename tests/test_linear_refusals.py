@@ -39,6 +39,15 @@ def test_fuse_linears_leaves_hooks_and_subclasses():
     assert type(net[0]) is Mine and net[1] is hooked and net[2].activation == "none" and net[3] is act
     assert type(net[4]) is fused.LinearAct
 
+    class Branches(torch.nn.Sequential):
+        def forward(self, x):
+            return sum(m(x) for m in self)
+    assert type(fused.fuse_linears(Branches(torch.nn.Linear(3, 3), torch.nn.ReLU()))[0]) is torch.nn.Linear
+    assert type(fused.fuse_linears(torch.nn.Sequential(torch.nn.Linear(3, 3).double()))[0]) is torch.nn.Linear
+    back = torch.nn.Linear(3, 3)
+    back.register_full_backward_hook(lambda *a: None)
+    assert fused.fuse_linears(torch.nn.Sequential(back))[0] is back
+
 
 def test_c_entries_check_their_arguments():
     L = _native.lib()

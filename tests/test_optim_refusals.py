@@ -32,6 +32,14 @@ def test_bad_parameters_and_gradients():
         optim.AdamW([{"params": [p]}, {"params": [p]}])
 
 
+def test_state_is_not_made_inside_a_capture(monkeypatch):
+    p = _p(3)
+    opt = optim.AdamW([p])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError):
+        opt._init_state(p, opt.param_groups[0])
+
+
 def test_a_copied_optimiser_knows_its_parameters():
     import copy
     opt = copy.deepcopy(optim.AdamW([_p(3), _p(4)], state_bits=8))

@@ -24,6 +24,8 @@ def _args(**over):
     (dict(old_logp=torch.zeros(2)), ValueError),
     (dict(advantages=torch.zeros(2, 3, requires_grad=True)), ValueError),
     (dict(ref_logp=torch.zeros(3, 2)), ValueError),
+    (dict(old_logp=torch.zeros(2, 3, dtype=torch.float64)), TypeError),
+    (dict(advantages=torch.zeros(2, 3, dtype=torch.int64)), TypeError),
     (dict(mask=torch.zeros(2, 3)), TypeError),
     (dict(mask=torch.zeros(2, dtype=torch.bool)), ValueError),
     (dict(kl_coeff=0.1), ValueError),
