@@ -150,18 +150,18 @@ __device__ __forceinline__ void store8(T* p, int have, const float (&x)[8])
     }
 }
 
-// act's argument for the backward: fp32, or fp16 next to 16-bit tensors of either type.  fp16 keeps 11 bits where
-// bf16 keeps 8, so that the slope taken from it adds nothing to the rounding of dh itself (with bf16 the
-// gradients were 1.6 times as far from exact ones as their own type's rounding, so 1.4); beyond its
-// range every activation's slope is constant.
-template <class T> struct PreOf { typedef f16_t type; };
-template <> struct PreOf<float> { typedef float type; };
+// act's argument for the backward: fp32, next to bf16 tensors fp16.  The slope is taken from it, and its rounding must
+// not add to that of dh and of the gradient itself (two roundings, 1.41 times one): with bf16 the gradients of bf16
+// tensors were 1.6 times one rounding off, with fp16 those of fp16 tensors 1.52 times; with 3 bits more (fp16
+// next to bf16) and with fp32 1.42.  Beyond fp16's range every activation's slope is constant.
+template <class T> struct PreOf { typedef float type; };
+template <> struct PreOf<bf16_t> { typedef f16_t type; };
 template <class T>
 __device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const float (&x)[8])
 {
     float h[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = sizeof(T) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    for (int j = 0; j < 8; ++j) h[j] = sizeof(typename PreOf<T>::type) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
     store8(static_cast<typename PreOf<T>::type*>(pre) + at, have, h);
 }
 
@@ -985,7 +985,8 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
 #define ACT_BWD(T, H) hipLaunchKernelGGL((act_bwd_kernel<T, H>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
                                          static_cast<const H*>(h), reinterpret_cast<T*>(ws), n, act, aligned)
         if (kind == SMLVM_F32) ACT_BWD(float, float);
-        else if (kind == SMLVM_F16) ACT_BWD(f16_t, f16_t);
+        else if (kind == SMLVM_F16 && h_is_y) ACT_BWD(f16_t, f16_t);
+        else if (kind == SMLVM_F16) ACT_BWD(f16_t, float);
         else if (h_is_y) ACT_BWD(bf16_t, bf16_t);
         else ACT_BWD(bf16_t, f16_t);
 #undef ACT_BWD

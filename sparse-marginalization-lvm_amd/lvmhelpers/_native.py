@@ -806,7 +806,7 @@ def linear_fwd(x, w, bias, residual, act, want_pre):
     dt, dev = x.dtype, x.device
     kind = KINDS[dt]
     y = torch.empty((M, N), dtype=dt, device=dev)
-    pre = torch.empty((M, N), dtype=dt if dt == torch.float32 else torch.float16, device=dev) if want_pre else None
+    pre = torch.empty((M, N), dtype=torch.float16 if dt == torch.bfloat16 else torch.float32, device=dev) if want_pre else None
     L = lib()
     nbytes = L.smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None

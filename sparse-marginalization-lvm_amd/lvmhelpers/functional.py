@@ -272,7 +272,7 @@ def lowrank_categorical_nll(x, w, b, y):
 
 class _LinearAct(torch.autograd.Function):
     """act(x w^T + b) + r with the epilogue in the product's kernel.  For the backward the forward leaves
-    act's argument (float32, or float16 next to 16-bit tensors; relu without a residual keeps its output instead)."""
+    act's argument (float32, or float16 next to bfloat16 tensors; relu without a residual keeps its output instead)."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, act):
