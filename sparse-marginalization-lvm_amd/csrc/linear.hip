@@ -690,17 +690,30 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const GemmArgs g)
 
 // Joins the partial sums of a split product, in order, and runs the epilogue; the workgroups behind the
 // first `blocks` join the column sums.
-struct Join { int splits, blocks, sum_blocks; };
+struct Join {
+    int splits, blocks;               // of the partial products
+    const float* sums;                // partial column sums [parts][n], joined by sum_blocks workgroups
+    int parts, sum_blocks;
+    int64_t n;
+    void* sum_out;
+};
 template <class T>
 __device__ __forceinline__ void join_body(const GemmArgs& g, const Join& p, int id)
 {
     const int splits = p.splits, blocks = p.blocks;
-    if (id >= blocks) {
-        const int64_t m = (int64_t)(id - blocks) * 256 + threadIdx.x;
-        if (m >= g.M) return;
+    if (id >= blocks) {                                                  // 64 sums, every fourth part to a wave
+        __shared__ float quarter[4][64];
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int64_t m = (int64_t)(id - blocks) * 64 + lane;
         float s = 0.0f;
-        for (int z = 0; z < splits; ++z) s += g.colsum_part[(int64_t)z * g.M + m];
-        static_cast<T*>(g.colsum)[m] = (T)s;
+        if (m < p.n) {
+#pragma unroll 8
+            for (int z = wave; z < p.parts; z += 4) s += p.sums[(int64_t)z * p.n + m];
+        }
+        quarter[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && m < p.n)
+            static_cast<T*>(p.sum_out)[m] = (T)((quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]));
         return;
     }
     const int64_t per_row = (g.N + 7) / 8, total = g.M * per_row;
@@ -727,23 +740,68 @@ __global__ __launch_bounds__(256) void join_kernel(const GemmArgs g, const Join 
     else join_body<T>(g2, p2, id - first);
 }
 
-// dh = dy act'(h), H the type h is kept in; relu may be given y in the place of h (the sign is the same).
+template <bool V> struct Flag { static constexpr bool value = V; };
+
+// dh = dy act'(h), H the type h is kept in; relu may be given y in the place of h (the sign is the same).  The column
+// sums db come from here, before dh is rounded: sums of rounded values are one rounding further off.  A workgroup owns
+// 8 * groups columns (groups a power of two) of `rows` rows, 256 / groups rows at a time; sums [gridDim.y][N] are
+// joined in order later.
 template <class T, class H>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const T* __restrict__ dy, const H* __restrict__ h, T* __restrict__ dh,
-                                                      int64_t n, int act, int aligned)
+                                                      int64_t M, int64_t N, int act, int groups, int64_t rows,
+                                                      float* __restrict__ sums)
 {
-    const int64_t stride = (int64_t)gridDim.x * 256 * 8;
-    for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < n; at += stride) {
-        float x[8], y[8];
-        if (aligned && at + 8 <= n) {
-            load_vec<H, 8>(h + at, x);
-            load_vec<T, 8>(dy + at, y);
+    __shared__ float shared[256 * 8];
+    const int tx = threadIdx.x & (groups - 1), ty = threadIdx.x / groups, step = 256 / groups;
+    const int64_t n = ((int64_t)blockIdx.x * groups + tx) * 8;
+    const int have = n >= N ? 0 : N - n < 8 ? (int)(N - n) : 8;
+    const int64_t last = (int64_t)(blockIdx.y + 1) * rows < M ? (int64_t)(blockIdx.y + 1) * rows : M;
+    float total[8] = {};
+    const int64_t end = M * N, first = (int64_t)blockIdx.y * rows + ty;
+    auto walk = [&](auto even) {                                         // even: N is a multiple of 8
+        constexpr bool EVEN = decltype(even)::value;
+        // (the elements that a row's last lane reads too many are the next row's; the last row has none behind it)
+        auto fetch = [&](int64_t at, float (&x)[8], float (&y)[8]) {
+            const int width = EVEN || at + 8 <= end ? 8 : have;
+            load8(h + at, width, x);
+            load8(dy + at, width, y);
+        };
+        auto one = [&](float (&y)[8], const float (&x)[8], int64_t at) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= act_slope_f<sizeof(T) == 2>(act, x[j]);
-            store_vec<T, 8>(dh + at, y);
-        } else {
-            for (int j = 0; j < 8 && at + j < n; ++j) dh[at + j] = (T)((float)dy[at + j] * act_slope_f<sizeof(T) == 2>(act, (float)h[at + j]));
+            for (int j = 0; j < 8; ++j) {
+                y[j] *= act_slope_f<sizeof(T) == 2>(act, x[j]);
+                total[j] += y[j];
+            }
+            store8(dh + at, EVEN ? 8 : have, y);
+        };
+        constexpr int U = 4;                                             // rows in flight
+        int64_t m = first;
+        for (; m + (U - 1) * step < last; m += U * step) {
+            float x[U][8], y[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) fetch((m + u * step) * N + n, x[u], y[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) one(y[u], x[u], (m + u * step) * N + n);
         }
+        for (; m < last; m += step) {
+            float x[8], y[8];
+            fetch(m * N + n, x, y);
+            one(y, x, m * N + n);
+        }
+    };
+    if (have) {
+        if (N % 8 == 0) walk(Flag<true>{});
+        else walk(Flag<false>{});
+    }
+    if (!sums) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) shared[threadIdx.x * 8 + j] = total[j];
+    __syncthreads();
+    if (ty == 0 && have) {
+        for (int t = 1; t < step; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) total[j] += shared[(t * groups + tx) * 8 + j];
+        store8(sums + (int64_t)blockIdx.y * N + n, have, total);
     }
 }
 
@@ -831,6 +889,7 @@ struct Job {
     Plan p;
     bool direct;
     int layout;
+    Join sums;                                       // column sums that another kernel has left in parts
 };
 
 // Plans a product and takes what it needs of the workspace.
@@ -860,9 +919,16 @@ static int plan_job(Job& j, int kind, int layout, void* colsum, char*& ws, size_
 
 static Join join_of(const Job& j)
 {
-    if (j.p.splits <= 1) return Join{0, 0, 0};
-    const int64_t want = (j.g.M * ((j.g.N + 7) / 8) + 255) / 256;
-    return Join{j.p.splits, (int)(want < 8192 ? want : 8192), j.g.colsum ? (int)((j.g.M + 255) / 256) : 0};
+    Join r = {};
+    if (j.p.splits > 1) {
+        const int64_t want = (j.g.M * ((j.g.N + 7) / 8) + 255) / 256;
+        r.splits = j.p.splits;
+        r.blocks = (int)(want < 8192 ? want : 8192);
+        if (j.g.colsum) { r.sums = j.g.colsum_part; r.parts = j.p.splits; r.n = j.g.M; r.sum_out = j.g.colsum; }
+    }
+    if (j.sums.sum_out) { r.sums = j.sums.sums; r.parts = j.sums.parts; r.n = j.sums.n; r.sum_out = j.sums.sum_out; }
+    r.sum_blocks = r.sum_out ? (int)((r.n + 63) / 64) : 0;
+    return r;
 }
 
 // one product, or a layer's dx and dw
@@ -889,7 +955,7 @@ static int launch_jobs(const Job* jobs, int count, hipStream_t stream)
             else launch_gemm<T, true, true>(j.p, j.direct, j.g, stream);
         }
     }
-    const Join ja = join_of(a), jb = count == 2 ? join_of(b) : Join{0, 0, 0};
+    const Join ja = join_of(a), jb = count == 2 ? join_of(b) : Join{};
     const int64_t blocks = (int64_t)ja.blocks + ja.sum_blocks + jb.blocks + jb.sum_blocks;
     if (blocks) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a.g, ja, b.g, jb);
     return check_launch();
@@ -916,6 +982,29 @@ static size_t workspace_of(int kind, int64_t M, int64_t N, int64_t K, bool colsu
 // dh, in front of the products' partial sums
 static size_t act_bytes(int kind, int64_t M, int64_t N) { return ((size_t)M * N * kind_bytes(kind) + 15) & ~(size_t)15; }
 
+// How act_bwd_kernel covers [M, N]: columns by `across` workgroups, rows in `parts`, some 2048 workgroups in all
+// with 4 rows at least for a thread.
+struct ActPlan {
+    int groups;
+    int64_t across, parts, rows;
+    size_t bytes(int64_t N) const { return ((size_t)parts * N * sizeof(float) + 15) & ~(size_t)15; }
+};
+static ActPlan act_plan(int64_t M, int64_t N)
+{
+    ActPlan p = {1, 0, 0, 0};
+    if (M <= 0 || N <= 0) return p;
+    while (p.groups < 256 && p.groups * 8 < N) p.groups *= 2;
+    p.across = (N + p.groups * 8 - 1) / (p.groups * 8);
+    const int64_t least = (256 / p.groups) * 4, most = (M + least - 1) / least;
+    p.parts = (2048 + p.across - 1) / p.across;
+    if (p.parts > most) p.parts = most;
+    if (p.parts < 1) p.parts = 1;
+    p.rows = (M + p.parts - 1) / p.parts;
+    if (p.rows < 1) p.rows = 1;
+    p.parts = (M + p.rows - 1) / p.rows;
+    return p;
+}
+
 // 1: go on, negative: an error
 static int check_sizes(int kind, int64_t M, int64_t N, int64_t K)
 {
@@ -937,7 +1026,7 @@ extern "C" size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, in
 {
     if (check_sizes(kind, M, N, K) != 1) return 0;
     const size_t dx = workspace_of(kind, M, K, N, false), dw = workspace_of(kind, N, K, M, true);
-    return dx + dw + (act ? act_bytes(kind, M, N) : 0);
+    return dx + dw + (act ? act_bytes(kind, M, N) + act_plan(M, N).bytes(N) : 0);
 }
 
 extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -958,7 +1047,8 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
         else launch_few_rows<bf16_t>(g, (hipStream_t)stream);
         return check_launch();
     }
-    Job job = {g, {}, false, 0};
+    Job job = {};
+    job.g = g;
     char* ws = static_cast<char*>(workspace);
     const int rc = plan_job(job, kind, 0, nullptr, ws, workspace_bytes);
     return rc == SMLVM_OK ? launch_kind(kind, &job, 1, (hipStream_t)stream) : rc;
@@ -976,14 +1066,15 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
         (dw && M && K && (!x || ldx < K))) return SMLVM_ERR_INVALID;
     const hipStream_t stream = (hipStream_t)stream_;
     char* ws = static_cast<char*>(workspace);
+    Join sums = {};
     if (act && some) {
-        const size_t bytes = act_bytes(kind, M, N);
+        const ActPlan p = act_plan(M, N);
+        const size_t held = act_bytes(kind, M, N), bytes = held + (db ? p.bytes(N) : 0);
         if (!ws || workspace_bytes < bytes) return SMLVM_ERR_WORKSPACE;
-        const int64_t n = M * N, need = (n + 2047) / 2048;
-        const dim3 grid((unsigned)(need < 16384 ? need : 16384));
-        const int aligned = aligned16(dy) && aligned16(h) && aligned16(ws);
+        float* const part = db ? reinterpret_cast<float*>(ws + held) : nullptr;
+        const dim3 grid((unsigned)p.across, (unsigned)p.parts);
 #define ACT_BWD(T, H) hipLaunchKernelGGL((act_bwd_kernel<T, H>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
-                                         static_cast<const H*>(h), reinterpret_cast<T*>(ws), n, act, aligned)
+                                         static_cast<const H*>(h), reinterpret_cast<T*>(ws), M, N, act, p.groups, p.rows, part)
         if (kind == SMLVM_F32) ACT_BWD(float, float);
         else if (kind == SMLVM_F16 && h_is_y) ACT_BWD(f16_t, f16_t);
         else if (kind == SMLVM_F16) ACT_BWD(f16_t, float);
@@ -992,23 +1083,23 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
 #undef ACT_BWD
         const int rc = check_launch();
         if (rc != SMLVM_OK) return rc;
+        if (db) { sums.sums = part; sums.parts = (int)p.parts; sums.n = N; sums.sum_out = db; }
         dy = ws;
         ws += bytes;
         workspace_bytes -= bytes;
     }
-    Job jobs[2];
+    Job jobs[2] = {};
     int count = 0, rc = SMLVM_OK;
     if (dx && M && K) {
         Job& j = jobs[count++];
-        j.g = GemmArgs{};
         j.g.a = dy; j.g.b = w; j.g.lda = ldy; j.g.ldb = ldw; j.g.M = M; j.g.N = K; j.g.K = N; j.g.out = dx;
         rc = plan_job(j, kind, 1, nullptr, ws, workspace_bytes);
     }
     if (rc == SMLVM_OK && N && (K ? dw != nullptr : db != nullptr)) {
         Job& j = jobs[count++];
-        j.g = GemmArgs{};
+        j.sums = sums;
         j.g.a = dy; j.g.b = x; j.g.lda = ldy; j.g.ldb = ldx; j.g.M = N; j.g.N = K; j.g.K = M; j.g.out = dw;
-        rc = plan_job(j, kind, 2, db, ws, workspace_bytes);
+        rc = plan_job(j, kind, 2, sums.sum_out ? nullptr : db, ws, workspace_bytes);
     }
     if (rc != SMLVM_OK || count == 0) return rc;
     return launch_kind(kind, jobs, count, stream);
