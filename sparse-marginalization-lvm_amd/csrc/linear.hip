@@ -424,8 +424,9 @@ struct Through {
 // BM x BN tile, WM x WN waves, DIRECT: 16-bit aligned operands.  Through registers one LDS buffer does: the next
 // tile waits in registers, and two or three workgroups per CU fill each other's gaps (two buffers of the fp32
 // planes would leave room for one).
+template <class T, int BM, int BN, bool DIRECT> constexpr int kBuffers = DIRECT || (sizeof(T) == 4 && BM == 256) ? 2 : 1;
 template <class T, int BM, int BN, bool DIRECT>
-constexpr int kLdsBytes = sizeof(T) == 4 ? 3 * (BM + BN) * 32 * 2 : (DIRECT ? 2 : 1) * (BM + BN) * 64 * 2;
+constexpr int kLdsBytes = kBuffers<T, BM, BN, DIRECT> * (BM + BN) * (sizeof(T) == 4 ? 3 * 32 : 64) * 2;
 
 // tile `id` of part `part_z`
 template <class T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, bool DIRECT>
@@ -439,7 +440,8 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
     using TA = Tile<BM, BK, ACOL>;
     using TB = Tile<BN, BK, BCOL>;
     constexpr int STAGE = PLANES * (TA::kBytes + TB::kBytes);
-    static_assert(kLdsBytes<T, BM, BN, DIRECT> == (DIRECT ? 2 : 1) * STAGE, "LDS");
+    constexpr int BUFFERS = kBuffers<T, BM, BN, DIRECT>;
+    static_assert(kLdsBytes<T, BM, BN, DIRECT> == BUFFERS * STAGE, "LDS");
 
     // (wave in a scalar register: matrix instructions ignore the exec mask, so what skips one has to be a
     // scalar branch)
@@ -547,24 +549,50 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
             sa.load(g.M - m0, k_end - k_begin, g.K - k_begin);
             sb.load(g.N - n0, k_end - k_begin, g.K - k_begin);
         }
-        for (int64_t s = 0; s < steps; ++s) {
-            __syncthreads();                                             // (the last tile has been read)
-            sa.store(lds);
-            sb.store(lds + PLANES * TA::kBytes);
-            __syncthreads();
-            if (s + 1 < steps) {
-                const int64_t left = k_end - k_begin - (s + 1) * BK, all = g.K - k_begin - (s + 1) * BK;
-                sa.load(g.M - m0, left, all);
-                sb.load(g.N - n0, left, all);
+        auto next = [&](int64_t step) {
+            const int64_t left = k_end - k_begin - step * BK, all = g.K - k_begin - step * BK;
+            sa.load(g.M - m0, left, all);
+            sb.load(g.N - n0, left, all);
+        };
+        auto put = [&](char* stage) {
+            sa.store(stage);
+            sb.store(stage + PLANES * TA::kBytes);
+        };
+        if constexpr (BUFFERS == 2) {
+            // The next tile is split and written while this one is multiplied: one barrier per step, and the
+            // vector work between the matrix instructions of the same wave (4096^3: 642 us as the compiler
+            // orders it, 592 as asked for below: 232 TFLOP/s, 1.39 PFLOP/s of bf16 products).
+            if (steps > 0) put(lds);
+            if (steps > 1) next(1);
+            for (int64_t s = 0; s < steps; ++s) {
+                __syncthreads();
+                compute(lds + (s & 1) * STAGE);
+                put(lds + ((s + 1) & 1) * STAGE);                        // (after the last step: what nobody reads)
+                // the order wanted: the step's LDS reads, then 4 matrix and 6 vector instructions in turn
+                __builtin_amdgcn_sched_group_barrier(0x100, PLANES * (FM * (ACOL ? 2 : 1) + FN * (BCOL ? 2 : 1)), 0);
+#pragma unroll
+                for (int i = 0; i < FM * FN * 6 / 4; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                    if (i % 2 == 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+                }
+                if (s + 2 < steps) next(s + 2);
             }
-            compute(lds);
+        } else {
+            for (int64_t s = 0; s < steps; ++s) {
+                __syncthreads();                                         // (the last tile has been read)
+                put(lds);
+                __syncthreads();
+                if (s + 1 < steps) next(s + 1);
+                compute(lds);
+            }
         }
     }
 
     // 16 rows at a time through the wave's own part of the LDS: a lane holds 4 n of one row, and stores 8 of
     // another, so that a row's stores fill whole cache lines.  (Rows 16 bytes apart in bank: no conflicts.)
     constexpr int COLS = BN / WN, PITCH = COLS + 4, PER_ROW = COLS / 8;
-    static_assert(WM * WN * 16 * PITCH * 4 <= (DIRECT ? 2 : 1) * STAGE, "epilogue tile");
+    static_assert(WM * WN * 16 * PITCH * 4 <= BUFFERS * STAGE, "epilogue tile");
     __syncthreads();
     float* const own = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
 #pragma unroll
@@ -812,21 +840,22 @@ struct Plan { int bm, bn, splits; int64_t k_split; };
 // tile, its own latency or its share of the CU, whichever is more; a split adds the join's launch and
 // its traffic.  The numbers are fits to products timed alone (us): 2048^3 bf16 with 64 / 128 / 256 tiles
 // 25.6 / 26.5 / 57.8; [53000 x 3920]^T [53000 x 128] fp32 with 64 tiles in 5 parts 499, with 128 tiles in 16
-// parts 344; [200 x 4000] [4000 x 4000]^T fp32 with 64 tiles whole 134, in 4 parts 63, with 128 tiles in 8 parts 53; [1 x 4096] [4096 x 4096]^T bf16 with 64 tiles whole 31, in 8 parts 10.7.
+// parts 344; [200 x 4000] [4000 x 4000]^T fp32 with 64 tiles whole 134, in 4 parts 63, with 128 tiles in 8 parts 53;
+// 4096^3 fp32 with 128 x 128 tiles 629, with 256 x 128 tiles 592; [1 x 4096] [4096 x 4096]^T bf16 with 64 tiles whole 31, in 8 parts 10.7.
 static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
 {
-    struct Tile { int size, slots; double fixed, latency, share; };
-    static const Tile kF32[] = {{128, 2, 5.0, 1.80, 1.14}, {64, 4, 3.0, 0.95, 0.45}};
-    static const Tile kDirect[] = {{256, 1, 14.0, 1.75, 1.75}, {128, 2, 5.0, 0.75, 0.60}, {64, 5, 2.5, 0.42, 0.18}};
-    static const Tile kThrough[] = {{128, 2, 6.0, 1.50, 0.95}, {64, 5, 3.0, 0.85, 0.27}};
+    struct Tile { int bm, bn, slots; double fixed, latency, share; };
+    static const Tile kF32[] = {{256, 128, 1, 9.0, 2.2, 2.2}, {128, 128, 2, 5.0, 1.80, 1.14}, {64, 64, 4, 3.0, 0.95, 0.45}};
+    static const Tile kDirect[] = {{256, 256, 1, 14.0, 1.75, 1.75}, {128, 128, 2, 5.0, 0.75, 0.60}, {64, 64, 5, 2.5, 0.42, 0.18}};
+    static const Tile kThrough[] = {{128, 128, 2, 6.0, 1.50, 0.95}, {64, 64, 5, 3.0, 0.85, 0.27}};
     const Tile* const set = kind == SMLVM_F32 ? kF32 : direct ? kDirect : kThrough;
-    const int sizes = kind == SMLVM_F32 ? 2 : direct ? 3 : 2;
+    const int sizes = kind == SMLVM_F32 || direct ? 3 : 2;
     const int64_t bk = kind == SMLVM_F32 ? 32 : 64, k_tiles = (K + bk - 1) / bk;
     Plan best = {64, 64, 1, bk};
     double least = 1e300;
     for (int i = 0; i < sizes; ++i) {
         const Tile& t = set[i];
-        const double tiles = (double)((M + t.size - 1) / t.size) * (double)((N + t.size - 1) / t.size);
+        const double tiles = (double)((M + t.bm - 1) / t.bm) * (double)((N + t.bn - 1) / t.bn);
         for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits / 2) {
             const int64_t per = k_tiles > 0 ? (k_tiles + splits - 1) / splits : 1;
             if (splits > 1 && per < 4) break;
@@ -837,7 +866,8 @@ static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
             if (splits > 1) time += 6.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
             if (time < least) {
                 least = time;
-                best.bm = best.bn = t.size;
+                best.bm = t.bm;
+                best.bn = t.bn;
                 best.k_split = per * bk;
                 best.splits = (int)(k_tiles > 0 ? (k_tiles + per - 1) / per : 1);
             }
@@ -863,6 +893,12 @@ static void launch_gemm(const Plan& p, bool direct, const GemmArgs& g, hipStream
             if (p.bm == 256) GEMM(256, 256, 2, 4, true);
             else if (p.bm == 128) GEMM(128, 128, 2, 2, true);
             else GEMM(64, 64, 2, 2, true);
+            return;
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (p.bm == 256) {
+            GEMM(256, 128, 4, 2, false);
             return;
         }
     }

@@ -119,6 +119,12 @@ def test_large_tiles_and_long_sums(dev, M, N, K, dtype):
     _check(dev, *_case(M, N, K, dtype, 1), "silu", dtype)
 
 
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 2048), (4100, 4090, 2050), (9000, 260, 9000)])
+def test_the_widest_fp32_tiles(dev, M, N, K):
+    """256 x 128 tiles with the next tile split while one is multiplied, full and partly filled."""
+    _check(dev, *_case(M, N, K, torch.float32, 1), "none", torch.float32)
+
+
 def test_fp32_keeps_fp32_accuracy(dev):
     """Values over 60 binades and sums that cancel: three bf16 parts carry all 24 bits."""
     g = torch.Generator().manual_seed(0)
