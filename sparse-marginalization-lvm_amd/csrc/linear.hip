@@ -480,7 +480,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
         const char* const tb = stage + PLANES * TA::kBytes;
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
-            if constexpr (FM * FN >= 32) __builtin_amdgcn_sched_barrier(0);   // (one step's operands at a time: registers)
+            if constexpr (FM * FN >= 32 && ACOL) __builtin_amdgcn_sched_barrier(0);   // (one step's operands at a time: registers)
             s16x8 af[PLANES][FM], bf[PLANES][FN];
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
@@ -515,6 +515,21 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
         }
     };
 
+    // The order wanted of a step of the largest 16-bit tiles: the first 32 k's LDS reads, then the second's among the
+    // first matrix instructions (8192 x 8192 x 4096: 455 -> 425 us, dx 443 -> 418; dw, whose reads are twice as
+    // many, has no registers left for it).
+    auto order = [&] {
+        if constexpr (DIRECT && FM * FN >= 32 && !ACOL) {
+            constexpr int READS = FM + FN * (BCOL ? 2 : 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, FM * FN / READS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * FM * FN - FM * FN / READS * READS, 0);
+        }
+    };
     const T* const a = static_cast<const T*>(g.a);
     const T* const b = static_cast<const T*>(g.b);
     const int64_t steps = k_end > k_begin ? (k_end - k_begin + BK - 1) / BK : 0;
@@ -539,6 +554,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
             wait_loads_and_sync();
             if (s + 1 < steps) issue(s + 1, (int)((s + 1) & 1));
             compute(lds + (s & 1) * STAGE);
+            order();
         }
     } else {
         Through<T, BM, BK, ACOL, THREADS> sa;
