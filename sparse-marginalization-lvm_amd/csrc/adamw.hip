@@ -17,6 +17,7 @@ constexpr int kTensors = 40;          // table entries a launch carries (72 B ea
 constexpr int kThreads = 256;
 constexpr int kLane = 8;              // consecutive elements per lane and pass
 constexpr int kPass = kThreads * kLane;
+constexpr int64_t kMostBlocks = 0xFFFFFF;   // a launch's threads stay below 2^32
 
 struct AdamwTable {
     smlvm_adamw_tensor t[kTensors];
@@ -296,7 +297,7 @@ extern "C" int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count
         if (t.n < 0) return SMLVM_ERR_INVALID;
         if (t.n && (!t.p || !t.g || !t.m || !t.v || !t.step)) return SMLVM_ERR_INVALID;
         if (t.n && state_bits == 8 && (!t.m_scale || !t.r_scale)) return SMLVM_ERR_INVALID;
-        if (t.n > ((int64_t)1 << 40)) return SMLVM_ERR_UNSUPPORTED;   // (workgroup numbers are 32 bits)
+        if (t.n > kMostBlocks * kPass) return SMLVM_ERR_UNSUPPORTED;
         most += t.n;
     }
     AdamwHyper hp;
@@ -318,7 +319,7 @@ extern "C" int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count
         for (; i < count && table.count < kTensors; ++i) {
             if (tensors[i].n == 0) continue;
             const uint64_t need = (uint64_t)((tensors[i].n + chunk - 1) / chunk);
-            if (blocks + need > 0x7FFFFFFFull && table.count) break;
+            if (blocks + need > kMostBlocks && table.count) break;
             table.t[table.count] = tensors[i];
             table.first[table.count++] = (uint32_t)blocks;
             blocks += need;

@@ -64,4 +64,7 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&x)[N]
     }
 }
 
+// A launch's threads along one axis stay below 2^32.
+inline bool grid_fits(double blocks, int threads) { return blocks * threads < 4294967296.0; }
+
 }  // namespace smlvm

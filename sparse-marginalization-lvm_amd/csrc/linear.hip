@@ -951,7 +951,8 @@ static int plan_job(Job& j, int kind, int layout, void* colsum, char*& ws, size_
     j.layout = layout;
     j.direct = direct_ok(kind, g.a, g.lda, layout == 2 ? g.M : g.K) && direct_ok(kind, g.b, g.ldb, layout ? g.N : g.K);
     j.p = plan(kind, g.M, g.N, g.K, j.direct);
-    if ((double)((g.M + j.p.bm - 1) / j.p.bm) * (double)((g.N + j.p.bn - 1) / j.p.bn) > 1.0e9) return SMLVM_ERR_UNSUPPORTED;
+    if (!grid_fits((double)((g.M + j.p.bm - 1) / j.p.bm) * (double)((g.N + j.p.bn - 1) / j.p.bn),
+                   j.p.bm == 256 ? 512 : 256)) return SMLVM_ERR_UNSUPPORTED;
     g.tiles_m = (int)((g.M + j.p.bm - 1) / j.p.bm);
     g.tiles_n = (int)((g.N + j.p.bn - 1) / j.p.bn);
     if (g.tiles_n == 0) g.tiles_n = 1;               // (column sums alone)
@@ -989,9 +990,12 @@ static int launch_jobs(const Job* jobs, int count, hipStream_t stream)
 {
     const Job& a = jobs[0];
     const Job& b = jobs[count - 1];
+    const Join ja = join_of(a), jb = count == 2 ? join_of(b) : Join{};
+    const int64_t blocks = (int64_t)ja.blocks + ja.sum_blocks + jb.blocks + jb.sum_blocks;
+    if (!grid_fits((double)blocks, 256)) return SMLVM_ERR_UNSUPPORTED;
     if (count == 2 && a.p.bm == 64 && b.p.bm == 64) {
         const int64_t blocks_a = (int64_t)a.g.tiles_m * a.g.tiles_n * a.p.splits, blocks_b = (int64_t)b.g.tiles_m * b.g.tiles_n * b.p.splits;
-        if (blocks_a + blocks_b > 0x7FFFFFFF) return SMLVM_ERR_UNSUPPORTED;
+        if (!grid_fits((double)(blocks_a + blocks_b), 256)) return SMLVM_ERR_UNSUPPORTED;
         const dim3 grid((unsigned)(blocks_a + blocks_b));
         if (sizeof(T) == 2 && a.direct && b.direct) {
             if constexpr (sizeof(T) == 2)
@@ -1007,8 +1011,6 @@ static int launch_jobs(const Job* jobs, int count, hipStream_t stream)
             else launch_gemm<T, true, true>(j.p, j.direct, j.g, stream);
         }
     }
-    const Join ja = join_of(a), jb = count == 2 ? join_of(b) : Join{};
-    const int64_t blocks = (int64_t)ja.blocks + ja.sum_blocks + jb.blocks + jb.sum_blocks;
     if (blocks) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a.g, ja, b.g, jb);
     return check_launch();
 }
@@ -1094,6 +1096,7 @@ extern "C" int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64
     g.a = x; g.b = w; g.lda = ldx; g.ldb = ldw; g.M = M; g.N = N; g.K = K;
     g.out = y; g.bias = bias; g.res = residual; g.ldr = ldr; g.pre = pre; g.act = act;
     if (M <= kFewRows) {
+        if (!grid_fits((double)((N + 7) / 8), 256)) return SMLVM_ERR_UNSUPPORTED;
         if (kind == SMLVM_F32) launch_few_rows<float>(g, (hipStream_t)stream);
         else if (kind == SMLVM_F16) launch_few_rows<f16_t>(g, (hipStream_t)stream);
         else launch_few_rows<bf16_t>(g, (hipStream_t)stream);

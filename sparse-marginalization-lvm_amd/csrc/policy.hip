@@ -223,7 +223,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void rows_kernel(const RowsIn in
     constexpr int BLOCK = G < 256 ? 256 : G;
     constexpr int P = kPer<T>;
     constexpr int U = R == 0 ? 4 : (R < 4 ? R : 4);     // vectors absorbed under one maximum
-    uint32_t row = blockIdx.x * (BLOCK / G) + threadIdx.x / G;
+    uint32_t row = (blockIdx.y * gridDim.x + blockIdx.x) * (BLOCK / G) + threadIdx.x / G;
     const bool live = row < in.rows;
     if (!live) row = in.rows - 1;                        // whole lane groups stay busy
     const int lane = threadIdx.x & (G - 1);
@@ -383,9 +383,14 @@ template <class T, bool POLICY, bool GRAD>
 static void launch_rows(const RowsIn& in, const RowsOut& out, const Policy& pol, hipStream_t stream)
 {
     const int64_t nv = ((int64_t)in.V + kPer<T> - 1) / kPer<T>;
+    // (in two axes: a launch's threads along one of them stay below 2^32)
+    auto grid = [&](uint32_t per) {
+        const uint32_t blocks = (in.rows + per - 1) / per, x = blocks < (1u << 21) ? blocks : 1u << 21;
+        return dim3(x, (blocks + x - 1) / x);
+    };
 #define ROWS(G, R)                                                                                             \
-    hipLaunchKernelGGL((rows_kernel<T, G, R, POLICY, GRAD>), dim3((in.rows + (G < 256 ? 256 / G : 1) - 1) /    \
-                       (G < 256 ? 256 / G : 1)), dim3(G < 256 ? 256 : G), 0, stream, in, out, pol)
+    hipLaunchKernelGGL((rows_kernel<T, G, R, POLICY, GRAD>), grid(G < 256 ? 256 / G : 1), dim3(G < 256 ? 256 : G), \
+                       0, stream, in, out, pol)
     if (nv <= 8) ROWS(8, 1);
     else if (nv <= 64) ROWS(64, 1);
     else if (nv <= 128) ROWS(64, 2);

@@ -380,3 +380,21 @@ def test_two_streams_and_bitwise_repeats(dev):
         torch.cuda.current_stream().wait_stream(s)
     for o in outs:
         assert all(torch.equal(x, y) for x, y in zip(first, o))
+
+
+@pytest.mark.parametrize("V,rows", [(200, (1 << 23) + 3), (1500, (1 << 21) + 5)])     # 4 rows and 1 row to a workgroup
+def test_rows_of_more_than_two_million_workgroups(V, rows, dev):
+    gen = torch.Generator().manual_seed(3)
+    z = torch.randn(1, V, generator=gen)
+    actions = torch.randint(0, V, (rows,), generator=gen)
+    logp, entropy = _F().token_logprobs(z.to(dev).expand(rows, V), actions.to(dev))
+    want = torch.log_softmax(z.double()[0], 0)
+    # (every row is the same: none may differ; to the formula 64 of fp32's half steps, of which a sum of 1500 terms in
+    # a tree, the exponentials and the logarithm take fewer than 40)
+    table = torch.full((V,), float("nan"), device=dev)
+    table[actions.to(dev)] = logp
+    assert torch.equal(table[actions.to(dev)], logp)
+    seen = torch.unique(actions)
+    assert (table.cpu()[seen].double() - want[seen]).abs().max() <= 2.0 ** -18 * want.abs().max()
+    assert torch.equal(entropy, entropy[:1].expand(rows))
+    assert abs(float(entropy[0]) + float((want.exp() * want).sum())) <= 2.0 ** -18 * abs(float((want.exp() * want).sum()))

@@ -77,3 +77,16 @@ def test_c_entries_check_their_arguments():
     assert bwd(act=2, h_is_y=1) == -1                                                          # y stands in for relu only
     assert bwd(ws=None) == -4 and bwd(nbytes=8) == -4
     assert bwd(dx=None, dw=None, db=None, act=0) == 0                                          # nothing wanted
+
+
+def test_launches_of_too_many_threads_are_refused():
+    L = _native.lib()
+    i64, i32 = ctypes.c_int64, ctypes.c_int32
+    one, most = ctypes.c_void_p(16), (1 << 31) - 1
+    for kind in (0, 1, 2):
+        for M, N in ((1, most), (4, most), (most, 1)):
+            assert L.smlvm_linear_fwd_workspace_bytes(kind, M, N, 1) == 0
+            assert L.smlvm_linear_fwd(one, i64(1), one, i64(1), None, None, i64(N), one, None, i32(kind), i32(0), i64(M), i64(N),
+                                      i64(1), None, ctypes.c_size_t(0), None) == -2
+        assert L.smlvm_linear_bwd(one, i64(1), None, i32(0), one, i64(1), one, i64(1), one, None, None, i32(kind), i32(0),
+                                  i64(most), i64(1), i64(1), None, ctypes.c_size_t(0), None) == -2

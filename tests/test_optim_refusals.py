@@ -66,3 +66,12 @@ def test_c_entry_checks_its_arguments():
     assert call(pack(16, 16, 16, 16, 0, 16, 16, 5, 0), bits=8) == -1
     assert call(pack(16, 16, 16, 16, 0, 0, 16, (1 << 40) + 1, 0)) == -2
     assert call(pack(16, 16, 16, 16, 0, 0, 16, (1 << 64) - 1, 0)) == -1       # n = -1
+
+
+def test_a_tensor_of_too_many_workgroups_is_refused():
+    L = _native.lib()
+    d, f, i32 = ctypes.c_double, ctypes.c_float, ctypes.c_int32
+    for bits in (32, 8):
+        entry = _native.ADAMW_ENTRY.pack(16, 16, 16, 16, 16, 16, 16, 1 << 35, 0)      # 2^24 workgroups of 256 threads
+        assert L.smlvm_adamw_step(ctypes.c_char_p(entry), i32(1), i32(0), i32(0), i32(bits), d(0.9), d(0.999), f(1e-8),
+                                  f(1e-3), None, f(0.0), ctypes.c_uint32(0), ctypes.c_void_p(16), None) == -2
