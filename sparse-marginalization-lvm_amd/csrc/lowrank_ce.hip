@@ -9,7 +9,7 @@
 //
 //   fwd   lane = two (row, feature) pairs: one exp pass over the C classes, shifted by an upper
 //         bound of the logits (exact two-pass redo if that underflows); W and b are read with
-//         wave-uniform addresses (scalar loads) and feed v_pk_fma_f32; then a per-row sum.
+//         wave-uniform addresses (scalar loads) and feed both pairs' FMAs; then a per-row sum.
 //   bwd   dX: lane = one (row, feature), softmax from the saved lse, dX = g (softmax - onehot) W
 //         dW, db: thread = one class, loops over (row, feature) tiles staged in LDS; per-block
 //         partials, then a deterministic fp64 reduction over blocks (no float atomics).
@@ -40,9 +40,8 @@ __device__ __forceinline__ int label_at(const void* y, int64_t i, int C)
     return (v >= 0 && v < (long long)C) ? (int)v : -1;
 }
 
-// Every lane carries TWO (row, feature) pairs -- p and p + 256 of the block's 512 -- so that the
-// R FMAs of a logit and the shift run as v_pk_fma_f32 with the (wave-uniform) weight in a scalar
-// register; only the v_exp_f32 are per element.
+// Every lane carries TWO (row, feature) pairs -- p and p + 256 of the block's 512 -- so that
+// a (wave-uniform) weight, once in a scalar register, serves two of the R FMAs of a logit and of the shift.
 template <int R>
 __device__ __forceinline__ f32x2 logit2(const f32x2 (&x)[R], const float* __restrict__ w,
                                         const float* __restrict__ b, int c)
@@ -99,8 +98,8 @@ __device__ void dxdir_exact(const f32x2 (&x)[R], int half, const float* __restri
 
 constexpr int kPixPerBlock = 512;
 
-// DXD (round 3): the pass that sums exp(logit - bound) also sums exp(logit - bound) W[c, :], R more
-// packed FMAs per class; divided by the first sum that is softmax . W, and
+// DXD: the pass that sums exp(logit - bound) also sums exp(logit - bound) W[c, :], R more
+// FMAs per class and pair; divided by the first sum that is softmax . W, and
 //     dxdir[p, :] = sum_c softmax_c W[c, :] - W[y_p, :]
 // is the gradient of the element's loss with respect to x[p, :].  The backward's dX is then
 // gloss[n] * dxdir -- the dX kernel and its whole exp pass (one of the step's three) are gone.

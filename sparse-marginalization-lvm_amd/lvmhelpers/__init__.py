@@ -9,6 +9,14 @@ package for the sparse-marginalization path:
     lvmhelpers.pbinary_topk / pbernoulli / pbudget   the former Cython oracles
     lvmhelpers.utils       DeterministicWrapper, populate_common_params
 
+Next to it, what else a training step of such models runs (no counterpart in the reference, which uses
+torch's own):
+
+    lvmhelpers.functional  linear_act, token_logprobs, clipped_policy_loss
+    lvmhelpers.fused       LinearAct, fuse_linears (besides the decoder loss and the hoisted receiver)
+    lvmhelpers.optim       AdamW, with 32- or 8-bit states
+    lvmhelpers.graphs      GraphedStep: the whole step as one HIP graph
+
 The arithmetic runs in hand-written gfx950 HIP kernels behind the C ABI of
 ``include/sparsemarg.h`` (``lvmhelpers._native``); there is no CPU fallback.
 

@@ -2,8 +2,7 @@
 
 No counterpart in the reference (its steps run eagerly under PyTorch Lightning).  At the reference's
 batch size of 64 a step of the structured estimators is ~60 kernel launches of a few microseconds
-each and the GPU idles between them (1.4-2.6 ms per step with the device a few per
-cent busy); replayed as one graph the same launches go out back to back.
+each and the GPU idles between them (1.4-2.6 ms per step with the device a few per cent busy); replayed as one graph the same launches go out back to back.
 
 What makes a step capturable is that nothing in it depends on the data's SHAPE and nothing is read
 back: `TopKSparsemaxMarg`, `SparseMAPWrapper` / `SparseMAPMarg` have a `static_shapes` mode for that
@@ -11,7 +10,7 @@ back: `TopKSparsemaxMarg`, `SparseMAPWrapper` / `SparseMAPMarg` have a `static_s
 the support with weight 0 -- which `GraphedStep` switches on.  The kernels themselves are launched
 on the capturing stream like any other op, and their workspaces come from PyTorch's allocator,
 which gives a capture its own pool.  The optimiser must keep its state on the device
-(`torch.optim.Adam(..., capturable=True)`).
+(`lvmhelpers.optim.AdamW(...)`, or `torch.optim.Adam(..., capturable=True)`).
 
     step = GraphedStep(model, optimizer, first_batch)
     for batch in loader:
@@ -29,7 +28,7 @@ the same model and optimiser instead of raising.
 
 Limits: one process (no gradient all-reduce inside the graph); hyper-parameters that are Python
 numbers are baked in at capture -- a learning-rate schedule needs the rate as a tensor
-(`Adam(lr=torch.tensor(1e-3, device=...), capturable=True)`, updated in place); fixed batch shape (a last, smaller batch needs its own GraphedStep or an eager step); the
+(`AdamW(lr=torch.tensor(1e-3, device=...))`, updated in place); fixed batch shape (a last, smaller batch needs its own GraphedStep or an eager step); the
 static-shape mode pays for B * k (top-k) or B * (n + 1) (SparseMAP) decoder rows instead of the
 support's, which is the right trade where a step is launch bound and the wrong one where the
 decoder dominates (config 5: 1024 samples of 128 bits per GPU).
