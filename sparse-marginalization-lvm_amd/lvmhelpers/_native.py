@@ -1,10 +1,11 @@
 """ctypes binding of ``libsparsemarg_hip.so`` (C ABI: ``include/sparsemarg.h``) for torch tensors.
 
 PyTorch is only plumbing here: it owns device memory and the current HIP stream; every function
-below hands raw device pointers, sizes and that stream to the C ABI and returns torch tensors that
+below (and every node of csrc/autograd.cpp) hands raw device pointers, sizes and that stream to the C ABI and returns torch tensors that
 wrap the outputs.  There is NO fallback: if the library is missing or a call fails, this raises.
 """
 import ctypes
+import importlib.util
 import os
 import struct
 
@@ -13,7 +14,10 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "csrc", "libsparsemarg_hip.so")
 
+NODES_PATH = os.path.join(os.path.dirname(LIB_PATH), "sparsemarg_autograd.so")
+
 _lib = None
+_nodes = None
 
 ABI_SYMBOLS = [
     "smlvm_abi_version", "smlvm_error_string", "smlvm_last_hip_error", "smlvm_graph_memsets_to_kernels", "smlvm_support_segment_sum", "smlvm_support_compact_fused_masks",
@@ -87,6 +91,20 @@ def lib():
             raise NativeError("libsparsemarg_hip.so: ABI version mismatch")
         _lib = L
     return _lib
+
+
+def autograd():
+    """The autograd nodes of csrc/autograd.cpp (loaded once): linear_act, token_logprobs, clipped_policy_loss."""
+    global _nodes
+    if _nodes is None:
+        lib()
+        if not os.path.exists(NODES_PATH):
+            raise NativeError(f"{NODES_PATH} not found: build it with `make -C sparse-marginalization-lvm_amd/csrc`")
+        spec = importlib.util.spec_from_file_location("sparsemarg_autograd", NODES_PATH)
+        nodes = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(nodes)
+        _nodes = nodes
+    return _nodes
 
 
 def _check(rc, what):
@@ -781,144 +799,15 @@ def segmented_logsumexp(v, row_offsets, shift=0.0):
     return out
 
 
-# ----------------------------------------------------------------------------------- linear layers
+# ----------------------------------------------------------------------------------- layers and policy loss
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4, "tanh": 5}
 
 
-def _rows(t, width):
-    """A matrix whose rows are consecutive elements (any distance apart) -> (tensor, row stride)."""
-    if t.is_contiguous():
-        return t, width
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < width:
-        t = t.contiguous()
-    return t, max(t.stride(0), width)
-
-
-def linear_fwd(x, w, bias, residual, act, want_pre):
-    """x [M,K], w [N,K], bias [N] or None, residual [M,N] or None, all of one type on one GPU ->
-    (y [M,N], pre [M,N] or None)."""
-    (M, K), N = x.shape, w.shape[0]
-    x, ldx = _rows(x, K)
-    w, ldw = _rows(w, K)
-    ldr = N
-    if residual is not None:
-        residual, ldr = _rows(residual, N)
-    dt, dev = x.dtype, x.device
-    kind = KINDS[dt]
-    y = torch.empty((M, N), dtype=dt, device=dev)
-    pre = torch.empty((M, N), dtype=torch.float16 if dt == torch.bfloat16 else torch.float32, device=dev) if want_pre else None
-    L = lib()
-    nbytes = L.smlvm_linear_fwd_workspace_bytes(kind, M, N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev):
-        _check(L.smlvm_linear_fwd(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, _ptr(y), _ptr(pre),
-                                      kind, act, M, N, K, _ptr(ws),
-                                      nbytes, _stream_ptr()), "smlvm_linear_fwd")
-    return y, pre
-
-
-def linear_bwd(dy, h, h_is_y, x, w, act, want_dx, want_dw, want_db):
-    """dy [M,N], h = pre of linear_fwd, or y (h_is_y: relu without a residual), None for act 0 ->
-    (dx, dw, db), each None unless wanted."""
-    (M, K), N = x.shape, w.shape[0]
-    dev, dt, kind = x.device, x.dtype, KINDS[x.dtype]
-    dy, ldy = (dy.contiguous(), N) if act else _rows(dy, N)
-    x, ldx = _rows(x, K)
-    w, ldw = _rows(w, K)
-    dx = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
-    dw = torch.empty((N, K), dtype=dt, device=dev) if want_dw or want_db else None
-    db = torch.empty(N, dtype=dt, device=dev) if want_db else None
-    nbytes = lib().smlvm_linear_bwd_workspace_bytes(kind, act, M, N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev):
-        _check(lib().smlvm_linear_bwd(_ptr(dy), ldy, _ptr(h), 1 if h_is_y else 0, _ptr(x), ldx, _ptr(w), ldw,
-                                      _ptr(dx), _ptr(dw), _ptr(db), kind, act, M, N, K, _ptr(ws),
-                                      nbytes, _stream_ptr()), "smlvm_linear_bwd")
-    return dx, (dw if want_dw else None), db
-
-
-# ----------------------------------------------------------------------------------- policy loss
-def _need_rows(logits):
-    """logits [B, T, V], one row's elements consecutive (B and T in any stride: a shifted slice of a
-    model's output is read where it lies)."""
+def need_logits(logits):
     if not logits.is_cuda:
         raise NativeError("logits: expected a GPU tensor (the hot path has no CPU fallback)")
     if logits.dtype not in KINDS:
         raise TypeError(f"logits: expected float32, float16 or bfloat16, got {logits.dtype}")
-    if logits.shape[2] > 1 and logits.stride(2) != 1:
-        logits = logits.contiguous()
-    return logits
-
-
-def _rows_args(logits, actions, mask):
-    return (_ptr(logits), KINDS[logits.dtype], logits.stride(0), logits.stride(1), _ptr(actions), _ptr(mask))
-
-
-def token_logprobs_fwd(logits, actions, mask=None, want_stats=True):
-    """logits [B,T,V], actions [B,T] int64, mask [B,T] uint8 or None -> (logp, entropy [B,T], stats [B,T,3])."""
-    logits = _need_rows(logits)
-    B, T, V = logits.shape
-    dev = logits.device
-    logp = torch.empty((B, T), dtype=torch.float32, device=dev)
-    entropy = torch.empty_like(logp)
-    stats = torch.empty((B, T, 3), dtype=torch.float32, device=dev) if want_stats else None
-    with _on(dev):
-        _check(lib().smlvm_token_logprobs_fwd(*_rows_args(logits, actions, mask), _ptr(logp), _ptr(entropy), _ptr(stats),
-                                              B, T, V, _stream_ptr()), "smlvm_token_logprobs_fwd")
-    return logp, entropy, stats
-
-
-def token_logprobs_bwd(logits, actions, mask, stats, c, h, g=None, out=None):
-    """dlogits [B,T,V] = g (c dlogp + h dentropy); stats, c, h: tensors, or addresses of such; out: a buffer
-    that holds the result for g = 1 already (it is written only where g is another number)."""
-    logits = _need_rows(logits)
-    B, T, V = logits.shape
-    keep = 0 if out is None else 1
-    if out is None:
-        out = torch.empty((B, T, V), dtype=logits.dtype, device=logits.device)
-    stats, c, h = (t if t is None or isinstance(t, int) else t.data_ptr() for t in (stats, c, h))
-    with _on(logits.device):
-        _check(lib().smlvm_token_logprobs_bwd(*_rows_args(logits, actions, mask), stats, c, h, _ptr(g), keep, _ptr(out), B, T,
-                                              V, _stream_ptr()), "smlvm_token_logprobs_bwd")
-    return out
-
-
-def policy_kept(kept):
-    """(stats, c, h) of `policy_loss`'s `kept` as addresses for token_logprobs_bwd."""
-    rows, at = kept.numel() // 5, kept.data_ptr()
-    return at, at + 12 * rows, at + 16 * rows
-
-
-def policy_loss(logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff, entropy_coeff,
-                mean, want_grad):
-    """-> (loss [], logp, entropy, kl [B,T], clipped [B,T] bool, kept [5 B T], dlogits [B,T,V] or None); `kept` is what
-    the backward needs (policy_kept)."""
-    logits = _need_rows(logits)
-    B, T, V = logits.shape
-    dev = logits.device
-    rows = B * T
-    logp, entropy, kl = torch.empty((3, B, T), dtype=torch.float32, device=dev).unbind(0)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    kept = torch.empty(rows * 5, dtype=torch.float32, device=dev)        # stats [rows, 3], c [rows], h [rows]
-    stats, c, h = policy_kept(kept)
-    clipped = torch.empty((B, T), dtype=torch.bool, device=dev)
-    dlogits = torch.empty((B, T, V), dtype=logits.dtype, device=dev) if want_grad else None
-    nbytes = 8 * (rows + 1)                                              # smlvm_policy_loss_workspace_bytes
-    ws = torch.empty(rows + 1, dtype=torch.float64, device=dev)
-    with _on(dev):
-        _check(lib().smlvm_policy_loss(
-            *_rows_args(logits, actions, mask), _ptr(old_logp), _ptr(advantages), _ptr(ref_logp), clip_low, clip_high,
-            kl_coeff, entropy_coeff, 1 if mean else 0, loss.data_ptr(), logp.data_ptr(), entropy.data_ptr(), kl.data_ptr(),
-            clipped.data_ptr(), stats, c, h, _ptr(dlogits), B, T, V, ws.data_ptr(), nbytes, _stream_ptr()),
-            "smlvm_policy_loss")
-    return loss, logp, entropy, kl, clipped, kept, dlogits
-
-
-def capture_id():
-    """The id of the graph capture that the current stream is part of, 0 outside one."""
-    got = ctypes.c_uint64(0)
-    _check(lib().smlvm_stream_capture_id(_stream_ptr(), ctypes.byref(got)), "smlvm_stream_capture_id")
-    return got.value
 
 
 # ----------------------------------------------------------------------------------- AdamW

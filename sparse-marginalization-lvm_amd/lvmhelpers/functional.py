@@ -1,17 +1,7 @@
 """torch.autograd glue over the C-ABI kernels (``_native``).  Host-side plumbing only."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-
-
-def _once(backward):
-    """once_differentiable for a backward, at no cost (3 us) where no graph of the backward is wanted."""
-    guarded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
 
 
 def _patterns_written(x, p, mask):
@@ -270,32 +260,6 @@ def lowrank_categorical_nll(x, w, b, y):
     return _LowRankCE.apply(x.contiguous(), w.contiguous(), b.contiguous(), y)
 
 
-class _LinearAct(torch.autograd.Function):
-    """act(x w^T + b) + r with the epilogue in the product's kernel.  For the backward the forward leaves
-    act's argument (float32, or float16 next to bfloat16 tensors; relu without a residual keeps its output instead)."""
-
-    @staticmethod
-    def forward(ctx, x, w, b, r, act):
-        need = any(ctx.needs_input_grad[:3])
-        own_sign = act == 1 and r is None          # relu: y > 0 exactly where its argument is
-        y, pre = _native.linear_fwd(x, w, b, r, act, want_pre=need and act != 0 and not own_sign)
-        if need:
-            ctx.act, ctx.h_is_y = act, own_sign
-            ctx.save_for_backward(x, w, *([y if own_sign else pre] if act else []))
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        dx = dw = db = None
-        want_dx, want_dw, want_db, want_dr = ctx.needs_input_grad[:4]
-        if want_dx or want_dw or want_db:
-            x, w = ctx.saved_tensors[:2]
-            dx, dw, db = _native.linear_bwd(dy, ctx.saved_tensors[2] if ctx.act else None, ctx.h_is_y, x, w, ctx.act, want_dx,
-                                            want_dw, want_db)
-        return dx, dw, db, (dy if want_dr else None), None
-
-
 def linear_act(x, weight, bias=None, activation="none", residual=None):
     """activation(x @ weight.T + bias) + residual as one kernel (split over the inner axis: two).
 
@@ -329,75 +293,8 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         residual = residual.reshape(x.shape[0], weight.shape[0])
     if bias is not None:
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        y = _LinearAct.apply(x, weight, bias, residual, act)
-    else:
-        y = _native.linear_fwd(x, weight, bias, residual, act, False)[0]
+    y = _native.autograd().linear_act(x, weight, bias, residual, act)
     return y if len(out_shape) == 2 else y.view(out_shape)
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    """(log softmax(logits)[action], entropy) per row without the [.., V] log-probabilities."""
-
-    @staticmethod
-    def forward(ctx, logits, actions, mask):
-        want = ctx.needs_input_grad[0]
-        ctx.set_materialize_grads(False)
-        logp, entropy, stats = _native.token_logprobs_fwd(logits, actions, mask, want_stats=want)
-        if want:
-            ctx.has_mask = mask is not None
-            ctx.save_for_backward(logits, actions, stats, *([mask] if mask is not None else []))
-        return logp, entropy
-
-    @staticmethod
-    @_once
-    def backward(ctx, glogp, gentropy):
-        logits, actions, stats = ctx.saved_tensors[:3]
-        mask = ctx.saved_tensors[3] if ctx.has_mask else None
-        if glogp is None and gentropy is None:
-            return None, None, None
-        c = torch.zeros_like(gentropy) if glogp is None else glogp
-        return _native.token_logprobs_bwd(logits, actions, mask, stats, c.contiguous(),
-                                          None if gentropy is None else gentropy.contiguous()), None, None
-
-
-class _ClippedPolicyLoss(torch.autograd.Function):
-    """The loss, and in the same pass over the logits its gradient.  The backward hands that buffer on
-    and only launches a kernel that returns at once when the incoming gradient is 1 and writes the
-    gradient anew from the logits when it is not (scaling the stored one would round 16-bit
-    values twice, and lose what fp16 had already flushed to zero).  The buffer is good for one backward
-    pass: a second one (retain_graph), or one recorded into another graph capture than the forward
-    (whose replays need not follow a replay of the forward), computes into a new tensor."""
-
-    @staticmethod
-    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coeff,
-                entropy_coeff, mean):
-        want = ctx.needs_input_grad[0]
-        ctx.set_materialize_grads(False)      # (no zeros for the statistics' gradients)
-        loss, logp, entropy, kl, clipped, kept, dlogits = _native.policy_loss(
-            logits, actions, mask, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coeff, entropy_coeff, mean, want)
-        if want:
-            ctx.has_mask = mask is not None
-            ctx.save_for_backward(logits, actions, kept, *([mask] if mask is not None else []))
-            ctx.ready = dlogits
-            ctx.capture = _native.capture_id()
-        ctx.mark_non_differentiable(logp, entropy, kl, clipped)
-        return loss, logp, entropy, kl, clipped
-
-    @staticmethod
-    @_once
-    def backward(ctx, g, *_):
-        if g is None:
-            return (None,) * 11
-        logits, actions, kept = ctx.saved_tensors[:3]
-        mask = ctx.saved_tensors[3] if ctx.has_mask else None
-        ready, ctx.ready = ctx.ready, None
-        if ready is not None and _native.capture_id() != ctx.capture:
-            ready = None
-        dlogits = _native.token_logprobs_bwd(logits, actions, mask, *_native.policy_kept(kept),
-                                             g=g.to(torch.float32).contiguous(), out=ready)
-        return (dlogits,) + (None,) * 10
 
 
 def _policy_rows(logits, actions, name):
@@ -450,10 +347,8 @@ def token_logprobs(logits, actions, mask=None):
     rows, act = _policy_rows(logits, actions, "token_logprobs")
     lead = logits.shape[:-1]
     mask = _row_mask(mask, lead, rows, "token_logprobs")
-    if torch.is_grad_enabled() and rows.requires_grad:
-        logp, entropy = _TokenLogprobs.apply(rows, act, mask)
-    else:
-        logp, entropy, _ = _native.token_logprobs_fwd(rows, act, mask, want_stats=False)
+    _native.need_logits(rows)
+    logp, entropy = _native.autograd().token_logprobs(rows, act, mask)
     return logp.view(lead), entropy.view(lead)
 
 
@@ -487,8 +382,10 @@ def clipped_policy_loss(logits, actions, old_logp, advantages, ref_logp=None, ma
     old = _row_values(old_logp, lead, rows, name, "old_logp", f32)
     adv = _row_values(advantages, lead, rows, name, "advantages", f32)
     ref = None if ref_logp is None else _row_values(ref_logp, lead, rows, name, "ref_logp", f32)
-    loss, logp, entropy, kl, clipped = _ClippedPolicyLoss.apply(
-        rows, act, old, adv, ref, _row_mask(mask, lead, rows, name), float(clip_low), float(clip_high),
+    mask = _row_mask(mask, lead, rows, name)
+    _native.need_logits(rows)
+    loss, logp, entropy, kl, clipped = _native.autograd().clipped_policy_loss(
+        rows, act, old, adv, ref, mask, float(clip_low), float(clip_high),
         float(kl_coeff), float(entropy_coeff), reduction == "mean")
     stats = {"logp": logp, "entropy": entropy, "kl": kl, "clipped": clipped}
     return loss, stats if len(lead) == 2 else {k: v.view(lead) for k, v in stats.items()}
