@@ -1,10 +1,10 @@
-// The autograd nodes of the layers, the log-probabilities and the policy loss, over the C ABI of
-// include/sparsemarg.h.  Host side only: output allocation, what is kept for the backward, the calls.
+// The autograd nodes of the layers, the log-probabilities and the policy loss, and the optimiser's table, over the
+// C ABI of include/sparsemarg.h.  Host side only: output allocation, what is kept for the backward, the calls.
 //
-// In C++ because these operators train small models, where a step is host time: the engine runs a node's
+// In C++ because these operators train small models, where a step is host time.  The engine runs a node's
 // backward on a thread of its own, and a node written in Python has to hand the interpreter's lock over twice
 // for it (an empty one costs 59 us, forward and backward, where the kernels of a small layer take 10).
-// Arguments are checked by the callers, lvmhelpers/functional.py.
+// Arguments of the nodes are checked by their callers, lvmhelpers/functional.py.
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -20,15 +20,16 @@ using torch::autograd::Function;
 using torch::autograd::variable_list;
 typedef std::optional<Tensor> Maybe;
 
-int32_t kind_of(const Tensor& t)
+int32_t kind_of(at::ScalarType type)
 {
-    switch (t.scalar_type()) {
+    switch (type) {
         case at::kFloat: return SMLVM_F32;
         case at::kHalf: return SMLVM_F16;
         case at::kBFloat16: return SMLVM_BF16;
-        default: TORCH_CHECK_TYPE(false, "expected float32, float16 or bfloat16, got ", t.scalar_type());
+        default: TORCH_CHECK_TYPE(false, "expected float32, float16 or bfloat16, got ", type);
     }
 }
+int32_t kind_of(const Tensor& t) { return kind_of(t.scalar_type()); }
 
 struct NativeError : std::runtime_error { using std::runtime_error::runtime_error; };   // lvmhelpers._native.NativeError
 
@@ -302,6 +303,115 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> clipped_policy_loss(
     return {out[0], out[1], out[2], out[3], out[4]};
 }
 
+// ------------------------------------------------------------------------------------------------ AdamW
+constexpr int64_t kBlock = 256;                       // elements that share one scale of an 8-bit state
+
+bool floating(const Tensor& t)
+{
+    const auto k = t.scalar_type();
+    return k == at::kFloat || k == at::kHalf || k == at::kBFloat16;
+}
+
+Tensor entry_of(const pybind11::dict& state, const char* key)
+{
+    PyObject* const o = PyDict_GetItemString(state.ptr(), key);
+    return o && THPVariable_Check(o) ? THPVariable_Unpack(o) : Tensor();
+}
+
+void adamw_check(const Tensor& p, const Tensor& g)
+{
+    if (!p.is_cuda() || g.device() != p.device())
+        throw NativeError("AdamW: parameters and gradients must be on one GPU (there is no CPU fallback)");
+    TORCH_CHECK_TYPE(floating(p) && g.layout() == at::kStrided && floating(g) && g.sizes() == p.sizes(),
+                     "AdamW: a gradient must be a dense float32, float16 or bfloat16 tensor of the parameter's shape ", p.sizes(),
+                     ", got ", g.scalar_type(), " ", g.sizes(), " (", g.layout(), ")");
+}
+
+// One group of parameters: grads[i] None (the parameter is left alone) or its gradient, states[i] its state, numbers[i]
+// its number in the rounding hash; tickets: device -> the kernel's counter word.  One launch per device, types
+// and kind of state.
+void adamw_step(const pybind11::list& params, const pybind11::list& grads, const pybind11::list& states, const pybind11::list& numbers,
+                const pybind11::dict& tickets, const pybind11::object& lr, double beta1, double beta2, double eps,
+                double weight_decay, int64_t seed)
+{
+    struct Launch { at::Device device; at::ScalarType p, g; int32_t bits; std::vector<smlvm_adamw_tensor> table; };
+    const at::NoGradGuard no_grad;
+    std::vector<Launch> launches;
+    std::vector<Tensor> keep;                         // alive until the launch: updated parameters and relaid gradients
+    const size_t count = params.size();
+    keep.reserve(2 * count);
+    for (size_t i = 0; i < count; ++i) {
+        if (grads[i].is_none()) continue;
+        const Tensor p = THPVariable_Unpack(params[i].ptr());
+        if (p.numel() == 0) continue;
+        Tensor g = pybind11::cast<Tensor>(grads[i]);
+        adamw_check(p, g);
+        const pybind11::dict state = states[i];
+        const Tensor m = entry_of(state, "exp_avg"), step = entry_of(state, "step");
+        Tensor v = entry_of(state, "exp_avg_sq"), m_scale, r_scale;
+        const bool small = !v.defined();
+        if (small) {
+            v = entry_of(state, "exp_rms");
+            m_scale = entry_of(state, "exp_avg_scale");
+            r_scale = entry_of(state, "exp_rms_scale");
+        }
+        for (const Tensor& t : {m, v, step})
+            if (!t.defined() || t.device() != p.device()) throw NativeError("AdamW: a parameter's state is not on its GPU");
+        TORCH_CHECK_VALUE(m.sizes() == p.sizes() && v.sizes() == p.sizes() && m.strides() == p.strides() && v.strides() == p.strides(),
+                          "AdamW: a parameter changed its shape or memory order after its state was made");
+        const auto kind = small ? at::kFloat8_e4m3fn : at::kFloat;
+        TORCH_CHECK_TYPE(m.scalar_type() == kind && v.scalar_type() == kind && step.scalar_type() == at::kLong && step.numel() == 1,
+                         "AdamW: a parameter's state has other types than this optimiser made it with");
+        if (small) {
+            const int64_t blocks = (p.numel() + kBlock - 1) / kBlock;
+            for (const Tensor& t : {m_scale, r_scale})
+                TORCH_CHECK_VALUE(t.defined() && t.device() == p.device() && t.scalar_type() == at::kFloat && t.numel() == blocks &&
+                                  t.is_contiguous(), "AdamW: the scales of an 8-bit state do not fit its parameter");
+        }
+        if (g.strides() != p.strides()) {
+            const c10::DeviceGuard guard(p.device());
+            g = at::empty_like(p, p.options().dtype(g.scalar_type())).copy_(g);
+            keep.push_back(g);
+        }
+        Launch* to = nullptr;
+        for (Launch& l : launches)
+            if (l.device == p.device() && l.p == p.scalar_type() && l.g == g.scalar_type() && l.bits == (small ? 8 : 32)) to = &l;
+        if (!to) {
+            launches.push_back({p.device(), p.scalar_type(), g.scalar_type(), small ? 8 : 32, {}});
+            to = &launches.back();
+            to->table.reserve(count);
+        }
+        to->table.push_back({p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), static_cast<float*>(ptr(m_scale)),
+                             static_cast<float*>(ptr(r_scale)), static_cast<int64_t*>(step.data_ptr()), p.numel(),
+                             pybind11::cast<uint64_t>(numbers[i])});
+        keep.push_back(p);
+    }
+    const bool rate_tensor = THPVariable_Check(lr.ptr());
+    for (const Launch& l : launches) {
+        const c10::DeviceGuard guard(l.device);
+        Tensor rate;
+        double number = 0.0;
+        if (rate_tensor) {
+            rate = THPVariable_Unpack(lr.ptr());
+            if (rate.device() != l.device) {
+                TORCH_CHECK_VALUE(!rate.is_cuda(), "AdamW: a tensor lr must be on the parameters' device");
+                number = rate.item<double>();
+                rate = Tensor();
+            }
+        } else {
+            number = pybind11::cast<double>(lr);
+        }
+        const pybind11::object device = pybind11::cast(l.device);
+        if (!tickets.contains(device)) tickets[device] = at::zeros({1}, at::TensorOptions(l.device).dtype(at::kInt));
+        const Tensor ticket = pybind11::cast<Tensor>(tickets[device]);
+        check(smlvm_adamw_step(l.table.data(), (int32_t)l.table.size(), kind_of(l.p), kind_of(l.g), l.bits, beta1, beta2, (float)eps, (float)number, static_cast<const float*>(ptr(rate)), (float)weight_decay,
+                               (uint32_t)seed, static_cast<uint32_t*>(ticket.data_ptr()), stream_of(ticket)),
+              "smlvm_adamw_step");
+    }
+    // (a graph that had saved a parameter's old value finds out)
+    for (const Tensor& p : keep) if (!p.is_inference()) torch::autograd::impl::bump_version(p);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -316,4 +426,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("linear_act", &linear_act);
     m.def("token_logprobs", &token_logprobs);
     m.def("clipped_policy_loss", &clipped_policy_loss);
+    m.def("adamw_step", &adamw_step);
 }

@@ -94,7 +94,8 @@ def lib():
 
 
 def autograd():
-    """The autograd nodes of csrc/autograd.cpp (loaded once): linear_act, token_logprobs, clipped_policy_loss."""
+    """The autograd nodes of csrc/autograd.cpp (loaded once): linear_act, token_logprobs, clipped_policy_loss;
+    and adamw_step."""
     global _nodes
     if _nodes is None:
         lib()
@@ -130,16 +131,6 @@ def _stream():
     if _raw_stream is not None and _raw_device is not None:
         return ctypes.c_void_p(_raw_stream(_raw_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def _stream_ptr():
-    if _raw_stream is not None and _raw_device is not None:
-        return _raw_stream(_raw_device())
-    return torch.cuda.current_stream().cuda_stream
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 class _Noop:
@@ -812,17 +803,6 @@ def need_logits(logits):
 
 # ----------------------------------------------------------------------------------- AdamW
 ADAMW_ENTRY = struct.Struct("@8QQ")    # smlvm_adamw_tensor: p, g, m, v, m_scale, r_scale, step, n, index
-
-
-def adamw_step(entries, p_dtype, g_dtype, state_bits, betas, eps, lr, weight_decay, seed, ticket):
-    """One smlvm_adamw_step over `entries` (bytes: ADAMW_ENTRY records of tensors on the current
-    device); lr: a number, or a float32 GPU tensor of one element; ticket: int32 [1], zero."""
-    lr_dev = lr if isinstance(lr, torch.Tensor) else None
-    _check(lib().smlvm_adamw_step(
-        entries, len(entries) // ADAMW_ENTRY.size, KINDS[p_dtype], KINDS[g_dtype],
-        state_bits, betas[0], betas[1], eps,
-        0.0 if lr_dev is not None else lr, _ptr(lr_dev), weight_decay, seed & 0xFFFFFFFF,
-        _ptr(ticket), _stream_ptr()), "smlvm_adamw_step")
 
 
 # ----------------------------------------------------------------------------------- HIP graphs

@@ -46,14 +46,13 @@ class AdamW(torch.optim.Optimizer):
                  min_8bit_size=4096, seed=0):
         self._order = {}        # parameter -> its number in the rounding hash
         self._tickets = {}      # device -> the kernel's counter word (zero between steps)
-        self._checked = {}      # a parameter's number -> what was found of it and its state (_entry)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size, seed=seed, capturable=True))
 
     def __setstate__(self, state):      # unpickled or deep-copied
         super().__setstate__(state)
         self._order = {p: i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
-        self._tickets, self._checked = {}, {}
+        self._tickets = {}
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -152,79 +151,23 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW.step: grads must have one entry per parameter")
         at = 0
         for group in self.param_groups:
-            launches = {}
-            keep = []            # gradients in another memory order, laid out anew: alive until the launch
-            for p in group["params"]:
-                g = p.grad if grads is None else grads[at]
-                at += 1
+            params = group["params"]
+            if grads is None:
+                given = [p.grad for p in params]
+            else:
+                given = grads[at:at + len(params)]
+                at += len(params)
+            states = []
+            for p, g in zip(params, given):
                 if g is None or p.numel() == 0:
+                    states.append(None)
                     continue
-                key, entry = self._entry(p, g, group, keep, at - 1, grads is not None)
-                entries = launches.get(key)
-                if entries is None:
-                    launches[key] = entries = []
-                entries.append(entry)
-            for (dev, p_dtype, g_dtype, bits), entries in launches.items():
-                lr = group["lr"]
-                if isinstance(lr, torch.Tensor) and lr.device != dev:
-                    if lr.is_cuda:
-                        raise ValueError("AdamW: a tensor lr must be on the parameters' device")
-                    lr = float(lr)
-                ticket = self._tickets.get(dev)
-                if ticket is None:
-                    ticket = self._tickets[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
-                with _native._on(dev):
-                    _native.adamw_step(b"".join(entries), p_dtype, g_dtype, bits, group["betas"], group["eps"], lr,
-                                       group["weight_decay"], group["seed"], ticket)
+                st = self.state[p]
+                if "step" not in st:
+                    if not p.is_cuda:
+                        raise _native.NativeError("AdamW: parameters must be on a GPU (there is no CPU fallback)")
+                    st = self._init_state(p, group)
+                states.append(st)
+            _native.autograd().adamw_step(params, given, states, [self._order[p] for p in params], self._tickets, group["lr"],
+                                          *group["betas"], group["eps"], group["weight_decay"], group["seed"] & 0xFFFFFFFF)
         return loss
-
-    def _entry(self, p, g, group, keep, order, foreign):
-        """(launch key, table record) of a parameter.  Addresses are read anew every time; what a check has
-        found of the very same tensors (`_checked`) is not checked again: a small model's step is bound
-        by these lines."""
-        st = self.state[p]
-        if "step" not in st:
-            self._check(p, g)
-            st = self._init_state(p, group)
-        m = st["exp_avg"]
-        v = st.get("exp_avg_sq")
-        bits = 32
-        if v is None:
-            v, bits = st["exp_rms"], 8
-        stride = p.stride()
-        known = self._checked.get(order)
-        if known is None or known[0] is not p or known[1] is not m or known[2] is not v or known[3] != stride:
-            kinds = (torch.float32, torch.float32) if bits == 32 else (torch.float8_e4m3fn, torch.float8_e4m3fn)
-            if m.shape != p.shape or v.shape != p.shape or m.stride() != stride or v.stride() != stride:
-                raise ValueError("AdamW: a parameter changed its shape or memory order after its state was made")
-            if (m.dtype, v.dtype) != kinds or st["step"].dtype != torch.int64:
-                raise TypeError("AdamW: a parameter's state has other types than this optimiser made it with")
-            self._check(p, g)
-            self._checked[order] = known = (p, m, v, stride, p.numel(), self._order[p])
-        elif foreign or g.layout != torch.strided:       # (torch itself keeps .grad to its parameter's shape and device)
-            self._check(p, g)
-        if not (p.is_cuda and g.is_cuda and m.is_cuda and v.is_cuda and st["step"].is_cuda) or p.dtype not in _FLOATS:
-            raise _native.NativeError("AdamW: a parameter, its gradient or its state left the GPU, or changed its type")
-        if g.stride() != stride:
-            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
-            keep.append(g)
-        if bits == 8:
-            blocks = -(-known[4] // BLOCK)
-            if any(t.numel() != blocks or t.dtype != torch.float32 or not t.is_cuda
-                   for t in (st["exp_avg_scale"], st["exp_rms_scale"])):
-                raise ValueError("AdamW: the scales of an 8-bit state do not fit its parameter")
-            entry = _native.ADAMW_ENTRY.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
-                                             st["exp_avg_scale"].data_ptr(), st["exp_rms_scale"].data_ptr(),
-                                             st["step"].data_ptr(), known[4], known[5])
-        else:
-            entry = _native.ADAMW_ENTRY.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0,
-                                             st["step"].data_ptr(), known[4], known[5])
-        return (p.device, p.dtype, g.dtype, bits), entry
-
-    @staticmethod
-    def _check(p, g):
-        if not p.is_cuda or g.device != p.device:
-            raise _native.NativeError("AdamW: parameters and gradients must be on one GPU (there is no CPU fallback)")
-        if g.layout != torch.strided or g.dtype not in _FLOATS or g.shape != p.shape:
-            raise TypeError(f"AdamW: a gradient must be a dense float32, float16 or bfloat16 tensor of the "
-                            f"parameter's shape {tuple(p.shape)}, got {g.dtype} {tuple(g.shape)} ({g.layout})")

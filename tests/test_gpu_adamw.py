@@ -408,3 +408,27 @@ def test_inside_a_graphed_training_step(dev, bits):
         models.append(model)
     # the graphed step weighs every slot, the eager one the support: the same sums in another order
     assert all(abs(x - y) <= 1e-4 * abs(x) for x, y in zip(*losses))
+
+
+def test_a_graph_that_kept_a_weight_notices_the_step(dev):
+    w = torch.nn.Parameter(torch.ones(8, 8, device=dev))
+    opt = _optim().AdamW([w])
+    x = torch.ones(4, 8, device=dev, requires_grad=True)
+    y = x @ w.t()
+    w.grad = torch.ones_like(w)
+    before = w._version
+    opt.step()
+    assert w._version > before
+    with pytest.raises(RuntimeError):           # dx = dy w needs the weight of before
+        y.sum().backward()
+
+
+def test_a_refused_gradient_leaves_every_parameter_alone(dev):
+    p, q = (torch.nn.Parameter(torch.ones(300, device=dev)) for _ in range(2))
+    opt = _optim().AdamW([p, q])
+    with pytest.raises(TypeError):
+        opt.step(grads=[torch.ones(300, device=dev), torch.ones(301, device=dev)])
+    torch.cuda.synchronize()
+    assert torch.equal(p, torch.ones_like(p)) and torch.equal(q, torch.ones_like(q))
+    opt.step(grads=[torch.ones(300, device=dev), torch.ones(300, device=dev)])
+    assert int(opt.state[p]["step"]) == 1 and int(opt.state[q]["step"]) == 1
