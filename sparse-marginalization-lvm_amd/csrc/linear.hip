@@ -167,14 +167,9 @@ __device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const
 
 // 8 consecutive n of row m: bias, activation, residual, stores
 template <class T>
-__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, float (&x)[8], int most = 8)
+__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, int have, float (&x)[8], const float (&b)[8], const float (&r)[8])
 {
-    const int have = g.N - n < most ? (int)(g.N - n) : most;
-    float r[8];
-    if (g.res) load8(static_cast<const T*>(g.res) + m * g.ldr + n, have, r);
     if (g.bias) {
-        float b[8];
-        load8(static_cast<const T*>(g.bias) + n, have, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += b[j];
     }
@@ -188,6 +183,15 @@ __device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n,
         for (int j = 0; j < 8; ++j) x[j] += r[j];
     }
     store8(static_cast<T*>(g.out) + m * g.N + n, have, x);
+}
+template <class T>
+__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n, float (&x)[8], int most = 8)
+{
+    const int have = g.N - n < most ? (int)(g.N - n) : most;
+    float r[8], b[8];
+    if (g.res) load8(static_cast<const T*>(g.res) + m * g.ldr + n, have, r);
+    if (g.bias) load8(static_cast<const T*>(g.bias) + n, have, b);
+    finish8<T>(g, m, n, have, x, b, r);
 }
 
 // ------------------------------------------------------------------------------------- staging
@@ -607,10 +611,26 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
 
     // 16 rows at a time through the wave's own part of the LDS: a lane holds 4 n of one row, and stores 8 of
     // another, so that a row's stores fill whole cache lines.  (Rows 16 bytes apart in bank: no conflicts.)
-    constexpr int COLS = BN / WN, PITCH = COLS + 4, PER_ROW = COLS / 8;
+    constexpr int COLS = BN / WN, PITCH = COLS + 4, PER_ROW = COLS / 8, V = 16 * PER_ROW / 64;
     static_assert(WM * WN * 16 * PITCH * 4 <= BUFFERS * STAGE, "epilogue tile");
+    static_assert(64 % PER_ROW == 0, "a lane's columns stay the same");
     __syncthreads();
     float* const own = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
+    const int64_t n = n0 + nw + lane % PER_ROW * 8, m_first = m0 + mw + lane / PER_ROW;
+    const int have = n >= g.N ? 0 : g.N - n < 8 ? (int)(g.N - n) : 8;
+    // the bias is loaded once, the residual 16 rows ahead: a load's latency in front of every store is what it cost
+    float bias[8], ahead[V][8];
+    const bool finishes = !g.part;
+    if (finishes && g.bias && have) load8(static_cast<const T*>(g.bias) + n, have, bias);
+    auto fetch = [&](int i) {
+        if (!finishes || !g.res || !have) return;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t m = m_first + i * 16 + v * (64 / PER_ROW);
+            if (m < g.M) load8(static_cast<const T*>(g.res) + m * g.ldr + n, have, ahead[v]);
+        }
+    };
+    fetch(0);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         if constexpr (ACOL) {
@@ -624,15 +644,20 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g, int id, int part_z,
         for (int j = 0; j < FN; ++j)
             *reinterpret_cast<f32x4*>(own + (lane & 15) * PITCH + j * 16 + ((lane >> 4) << 2)) = acc[i][j];
         wave_lds_sync();
+        float x[V][8], r[V][8];
 #pragma unroll
-        for (int v = 0; v < 16 * PER_ROW / 64; ++v) {
-            const int row = (v * 64 + lane) / PER_ROW, col = ((v * 64 + lane) % PER_ROW) * 8;
-            float x[8];
-            load_vec<float, 8>(own + row * PITCH + col, x);
-            const int64_t m = m0 + mw + i * 16 + row, n = n0 + nw + col;
-            if (m < g.M && n < g.N) {
-                if (g.part) store8(g.part + ((int64_t)part_z * g.M + m) * g.N + n, g.N - n < 8 ? (int)(g.N - n) : 8, x);
-                else finish8<T>(g, m, n, x);
+        for (int v = 0; v < V; ++v) {
+            load_vec<float, 8>(own + (v * (64 / PER_ROW) + lane / PER_ROW) * PITCH + lane % PER_ROW * 8, x[v]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[v][j] = ahead[v][j];
+        }
+        if (i + 1 < FM) fetch(i + 1);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t m = m_first + i * 16 + v * (64 / PER_ROW);
+            if (m < g.M && have) {
+                if (g.part) store8(g.part + ((int64_t)part_z * g.M + m) * g.N + n, have, x[v]);
+                else finish8<T>(g, m, n, have, x[v], bias, r[v]);
             }
         }
         wave_lds_sync();
