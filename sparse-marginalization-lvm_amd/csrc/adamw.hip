@@ -1,7 +1,8 @@
 // AdamW over many tensors at once, states in 32 or in 8 bits (formulas: include/sparsemarg.h).
 //
 // HBM bound: 28 B per element with fp32 weights, gradients and states (read p, g, m, v; write p, m,
-// v), 10 B with bf16 weights and gradients and 8-bit states.  Small models are launch bound instead,
+// v), 10 B with bf16 weights and gradients and 8-bit states.  Measured: 403M fp32 weights 2.06 ms (5.5 TB/s), 116M
+// bf16 weights with 8-bit states 252 us (4.6 TB/s, arithmetic taking about as long).  Small models are launch bound instead,
 // so one launch carries up to kTensors tensors: their table travels in the kernel arguments (no
 // device table to upload, nothing kept between calls, and a captured launch holds its own copy).
 // A workgroup owns kPass * passes consecutive elements of one tensor; a lane owns 8 of them at a time, so

@@ -16,6 +16,9 @@
 // products of order >= 2^-16 are summed in fp32 on the bf16 matrix cores: what is left out is
 // below 2^-23 of |x||w| per term, the size of fp32's own rounding.  Six bf16 products at 2.5 PFLOP/s
 // are 0.42 PFLOP/s, against 0.157 of the fp32 matrix instructions.
+//
+// Measured, [8192 x 4096] [8192 x 4096]^T bf16 with gelu and a residual: forward 530 us (425 the main loop, 1.29
+// PFLOP/s), dx 432, dw 459, dh 84; [53000 x 128] [3920 x 128]^T fp32: 384, 317 and 350 us.
 #include "elements.hpp"
 
 #include <math.h>
