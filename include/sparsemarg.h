@@ -378,7 +378,7 @@ int smlvm_graph_memsets_to_kernels(void* graph /* hipGraph_t */, int32_t* n_mems
  *   rounding.  Non-finite values become NaN codes.
  * `tensors` is a HOST array of `count` entries (read before the call returns).  No two entries may
  * share memory.  `ticket`: one device word, zero before the first call and left zero; calls that use
- * one ticket must not overlap.  lr_dev (nullable): the learning rate as a device float, read by the
+ * one ticket must not overlap.  A call that is captured into a graph does not use it (nullable there).  lr_dev (nullable): the learning rate as a device float, read by the
  * kernel instead of `lr`. */
 typedef struct {
     void* p;             /* [n] p_kind, updated in place */

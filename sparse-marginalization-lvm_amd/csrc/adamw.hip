@@ -248,7 +248,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamwTable table,
 
     // Every workgroup has read its step before it takes a number here (nothing else is ordered by the
     // ticket, so it is relaxed: a release would write the whole L2 back); the last one counts all
-    // the launch's tensors up and hands the ticket back at zero.
+    // the launch's tensors up and hands the ticket back at zero.  A captured launch has no ticket: its word would have
+    // to outlive every graph that holds it, and two graphs replayed side by side would share it.
     if (hp.ticket == nullptr) return;                            // (a kernel of its own counts up)
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -291,7 +292,10 @@ extern "C" int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count
     if (count < 0 || !kind_ok(p_kind) || !kind_ok(g_kind) || (state_bits != 32 && state_bits != 8)) return SMLVM_ERR_INVALID;
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return SMLVM_ERR_INVALID;
     if (count == 0) return SMLVM_OK;
-    if (!tensors || !ticket) return SMLVM_ERR_INVALID;
+    uint64_t capture = 0;
+    const int asked = smlvm_stream_capture_id(stream, &capture);
+    if (asked != SMLVM_OK) return asked;
+    if (!tensors || (!ticket && !capture)) return SMLVM_ERR_INVALID;
     int64_t most = 0;
     for (int i = 0; i < count; ++i) {
         const smlvm_adamw_tensor& t = tensors[i];
@@ -328,7 +332,7 @@ extern "C" int smlvm_adamw_step(const smlvm_adamw_tensor* tensors, int32_t count
         if (!table.count) break;
         table.first[table.count] = (uint32_t)blocks;
         // One word takes some 12 ns per workgroup: from 4096 on a second launch is cheaper.
-        hp.ticket = blocks <= 4096 ? ticket : nullptr;
+        hp.ticket = blocks <= 4096 && !capture ? ticket : nullptr;
         if (p_kind == SMLVM_F32) launch_g<float>(g_kind, state_bits, table, hp, (uint32_t)blocks, (hipStream_t)stream);
         else if (p_kind == SMLVM_F16) launch_g<f16_t>(g_kind, state_bits, table, hp, (uint32_t)blocks, (hipStream_t)stream);
         else launch_g<bf16_t>(g_kind, state_bits, table, hp, (uint32_t)blocks, (hipStream_t)stream);

@@ -328,9 +328,9 @@ void adamw_check(const Tensor& p, const Tensor& g)
 }
 
 // One group of parameters: grads[i] None (the parameter is left alone) or its gradient, states[i] its state, numbers[i]
-// its number in the rounding hash; tickets: device -> the kernel's counter word.  One launch per device, types
-// and kind of state.
-void adamw_step(const pybind11::list& params, const pybind11::list& grads, const pybind11::list& states, const pybind11::list& numbers,
+// its number in the rounding hash; tickets: device (its default stream) or (device, stream) -> the kernel's counter word.
+// One launch per device, types and kind of state.  True where a launch went into a graph capture.
+bool adamw_step(const pybind11::list& params, const pybind11::list& grads, const pybind11::list& states, const pybind11::list& numbers,
                 const pybind11::dict& tickets, const pybind11::object& lr, double beta1, double beta2, double eps,
                 double weight_decay, int64_t seed)
 {
@@ -387,6 +387,7 @@ void adamw_step(const pybind11::list& params, const pybind11::list& grads, const
         keep.push_back(p);
     }
     const bool rate_tensor = THPVariable_Check(lr.ptr());
+    bool captured = false;
     for (const Launch& l : launches) {
         const c10::DeviceGuard guard(l.device);
         Tensor rate;
@@ -401,15 +402,24 @@ void adamw_step(const pybind11::list& params, const pybind11::list& grads, const
         } else {
             number = pybind11::cast<double>(lr);
         }
-        const pybind11::object device = pybind11::cast(l.device);
-        if (!tickets.contains(device)) tickets[device] = at::zeros({1}, at::TensorOptions(l.device).dtype(at::kInt));
-        const Tensor ticket = pybind11::cast<Tensor>(tickets[device]);
+        const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(l.device.index());
+        uint64_t capture = 0;
+        check(smlvm_stream_capture_id(stream.stream(), &capture), "smlvm_stream_capture_id");
+        captured |= capture != 0;
+        Tensor ticket;                                // (a word per stream: steps on two of them may overlap)
+        if (!capture) {
+            pybind11::object key = pybind11::cast(l.device);
+            if (stream.id() != 0) key = pybind11::make_tuple(key, stream.id());
+            if (!tickets.contains(key)) tickets[key] = at::zeros({1}, at::TensorOptions(l.device).dtype(at::kInt));
+            ticket = pybind11::cast<Tensor>(tickets[key]);
+        }
         check(smlvm_adamw_step(l.table.data(), (int32_t)l.table.size(), kind_of(l.p), kind_of(l.g), l.bits, beta1, beta2, (float)eps, (float)number, static_cast<const float*>(ptr(rate)), (float)weight_decay,
-                               (uint32_t)seed, static_cast<uint32_t*>(ticket.data_ptr()), stream_of(ticket)),
+                               (uint32_t)seed, static_cast<uint32_t*>(ptr(ticket)), stream.stream()),
               "smlvm_adamw_step");
     }
     // (a graph that had saved a parameter's old value finds out)
     for (const Tensor& p : keep) if (!p.is_inference()) torch::autograd::impl::bump_version(p);
+    return captured;
 }
 
 }  // namespace

@@ -45,14 +45,14 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
                  min_8bit_size=4096, seed=0):
         self._order = {}        # parameter -> its number in the rounding hash
-        self._tickets = {}      # device -> the kernel's counter word (zero between steps)
+        self._tickets = {}      # device or (device, stream) -> the kernel's counter word (zero between steps)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size, seed=seed, capturable=True))
 
-    def __setstate__(self, state):      # unpickled or deep-copied
+    def __setstate__(self, state):      # unpickled, deep-copied, or from the base class's load_state_dict
         super().__setstate__(state)
         self._order = {p: i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
-        self._tickets = {}
+        self.__dict__.setdefault("_tickets", {})
 
     def add_param_group(self, group):
         super().add_param_group(group)

@@ -432,3 +432,34 @@ def test_a_refused_gradient_leaves_every_parameter_alone(dev):
     assert torch.equal(p, torch.ones_like(p)) and torch.equal(q, torch.ones_like(q))
     opt.step(grads=[torch.ones(300, device=dev), torch.ones(300, device=dev)])
     assert int(opt.state[p]["step"]) == 1 and int(opt.state[q]["step"]) == 1
+
+
+def test_steps_of_one_optimiser_on_two_streams(dev):
+    """Disjoint parameters of one optimiser, updated by two graphs on two streams and then by eager steps on them:
+    every step is counted, and the weights are an optimiser's that does one after the other."""
+    from lvmhelpers import graphs
+    n, k = 40, 20
+    a = [_param((3000 + i,), torch.float32, dev, i) for i in range(n)]
+    b = [p.clone() for p in a]
+    opt_a, opt_b = (_optim().AdamW(p, lr=1e-2, weight_decay=0.05) for p in (a, b))
+    grads = [_grad(p.shape, torch.float32, dev, i) for i, p in enumerate(a)]
+    halves = [[g if i % 2 == h else None for i, g in enumerate(grads)] for h in range(2)]
+    opt_a.step(grads=grads)
+    both = [graphs.capture(lambda h=h: opt_a.step(grads=halves[h]))[0] for h in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(k):
+        for s, graph in zip(streams, both):
+            with torch.cuda.stream(s):
+                graph.replay()
+    for _ in range(k):
+        for s, half in zip(streams, halves):
+            with torch.cuda.stream(s):
+                opt_a.step(grads=half)
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for _ in range(2 * k + 1):
+        opt_b.step(grads=grads)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and int(opt_a.state[p]["step"]) == 2 * k + 1

@@ -75,3 +75,10 @@ def test_a_tensor_of_too_many_workgroups_is_refused():
         entry = _native.ADAMW_ENTRY.pack(16, 16, 16, 16, 16, 16, 16, 1 << 35, 0)      # 2^24 workgroups of 256 threads
         assert L.smlvm_adamw_step(ctypes.c_char_p(entry), i32(1), i32(0), i32(0), i32(bits), d(0.9), d(0.999), f(1e-8),
                                   f(1e-3), None, f(0.0), ctypes.c_uint32(0), ctypes.c_void_p(16), None) == -2
+
+
+def test_load_state_dict_keeps_the_kernels_counter_words():
+    opt, word = optim.AdamW([_p(3)]), torch.zeros(1, dtype=torch.int32)
+    opt._tickets["here"] = word
+    opt.load_state_dict(optim.AdamW([_p(3)]).state_dict())
+    assert opt._tickets["here"] is word
