@@ -46,6 +46,7 @@ class AdamW(torch.optim.Optimizer):
                  min_8bit_size=4096, seed=0):
         self._order = {}        # parameter -> its number in the rounding hash
         self._tickets = {}      # device or (device, stream) -> the kernel's counter word (zero between steps)
+        self._captured = False  # a graph may hold the addresses of weights, states and rates
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size, seed=seed, capturable=True))
 
@@ -53,6 +54,7 @@ class AdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         self._order = {p: i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
         self.__dict__.setdefault("_tickets", {})
+        self.__dict__.setdefault("_captured", False)
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -117,14 +119,35 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As the base class, but every state keeps its own type (the base class casts floating
-        states to the parameter's) and is copied into the tensors that are there already, which
-        a captured step goes on using."""
+        states to the parameter's), and what a captured step uses stays where it is: values are copied
+        into the tensors of the states and of a tensor `lr` that are there already (a number that is loaded
+        for a tensor lr fills it).  Once a step has been captured, a state that state_dict does not have
+        starts anew in its own memory, and one of another kind (32 for 8 bits) is refused."""
         held = {p: dict(st) for p, st in self.state.items()}
+        rates = [g["lr"] for g in self.param_groups]
+        loaded = {p: state_dict["state"].get(i, {}) for g, saved in zip(self.param_groups, state_dict["param_groups"])
+                  for i, p in zip(saved["params"], g["params"])}
+        if self._captured:
+            for p, st in loaded.items():
+                if held.get(p) and st and any(not torch.is_tensor(st.get(k)) or st[k].shape != old.shape or st[k].dtype != old.dtype
+                                              for k, old in held[p].items()):
+                    raise ValueError("AdamW.load_state_dict: a captured step uses a state of another kind; load into a new optimiser")
+        first = {}
+        for rate, saved in zip(rates, state_dict["param_groups"]):
+            if torch.is_tensor(rate) and float(first.setdefault(id(rate), saved["lr"])) != float(saved["lr"]):
+                raise ValueError("AdamW.load_state_dict: groups that share one tensor lr would get different rates")
         super().load_state_dict(state_dict)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            for key, value in state_dict["state"].get(i, {}).items():
+        for group, rate in zip(self.param_groups, rates):
+            if torch.is_tensor(rate):
+                with torch.no_grad():
+                    rate.copy_(group["lr"]) if torch.is_tensor(group["lr"]) else rate.fill_(group["lr"])
+                group["lr"] = rate
+        for p, st in loaded.items():
+            if self._captured and held.get(p) and not st:
+                for old in held[p].values():
+                    old.zero_()
+                self.state[p] = held[p]
+            for key, value in st.items():
                 if not torch.is_tensor(value):
                     continue
                 old = held.get(p, {}).get(key)
@@ -168,6 +191,7 @@ class AdamW(torch.optim.Optimizer):
                         raise _native.NativeError("AdamW: parameters must be on a GPU (there is no CPU fallback)")
                     st = self._init_state(p, group)
                 states.append(st)
-            _native.autograd().adamw_step(params, given, states, [self._order[p] for p in params], self._tickets, group["lr"],
-                                          *group["betas"], group["eps"], group["weight_decay"], group["seed"] & 0xFFFFFFFF)
+            if _native.autograd().adamw_step(params, given, states, [self._order[p] for p in params], self._tickets, group["lr"],
+                                             *group["betas"], group["eps"], group["weight_decay"], group["seed"] & 0xFFFFFFFF):
+                self._captured = True
         return loss

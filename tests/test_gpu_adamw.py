@@ -463,3 +463,49 @@ def test_steps_of_one_optimiser_on_two_streams(dev):
         opt_b.step(grads=grads)
     for p, q in zip(a, b):
         assert torch.equal(p, q) and int(opt_a.state[p]["step"]) == 2 * k + 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_goes_on_after_load_state_dict(dev, bits):
+    """Replays after load_state_dict use the loaded states and rate and write no memory that was given back: the words
+    allocated after the load keep their values, and weights, states and counters are those of an eager twin."""
+    from lvmhelpers import graphs
+    shapes = [(300, 40), (40,), (5000,)]
+
+    def make(lr):
+        ps = [_param(s, torch.float32, dev, i) for i, s in enumerate(shapes)]
+        return ps, _optim().AdamW(ps, lr=lr, state_bits=bits, min_8bit_size=1, seed=3)
+    lr_a, lr_b = torch.full((), 1e-2, device=dev), torch.full((), 1e-2, device=dev)
+    (a, opt_a), (b, opt_b) = make(lr_a), make(lr_b)
+    c, opt_c = make(torch.full((), 3e-3, device=dev))          # what is loaded
+    grads = [_grad(s, torch.float32, dev, i) for i, s in enumerate(shapes)]
+    for _ in range(3):
+        opt_c.step(grads=grads)
+    for opt in (opt_a, opt_b):
+        opt.step(grads=grads)
+    graph, _ = graphs.capture(lambda: opt_a.step(grads=grads))
+    graph.replay()
+    opt_b.step(grads=grads)
+    saved = opt_c.state_dict()
+    opt_a.load_state_dict(saved)
+    opt_b.load_state_dict(saved)
+    words = [torch.full((1,), 7, dtype=torch.int32, device=dev) for _ in range(4096)]
+    for t in range(4):
+        for lr in (lr_a, lr_b):                                # a schedule goes on with the loaded rate
+            lr.mul_(0.5 if t else 1.0)
+        graph.replay()
+        torch.randn(1000, device=dev).sum().item()
+        opt_b.step(grads=grads)
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+            assert all(torch.equal(opt_a.state[p][k].float(), opt_b.state[q][k].float()) for k in opt_a.state[p])
+    assert int(opt_a.state[a[0]]["step"]) == 3 + 4 and abs(float(lr_a) - 3e-3 / 8) < 1e-9
+    assert bool((torch.stack(words) == 7).all())
+    # and with a state that holds nothing: the next replay is a fresh optimiser's first step
+    fresh, opt_f = make(1e-2)
+    for f, p in zip(fresh, a):
+        f.copy_(p)
+    opt_a.load_state_dict(opt_f.state_dict())
+    graph.replay()
+    opt_f.step(grads=grads)
+    assert all(torch.equal(p, f) for p, f in zip(a, fresh)) and int(opt_a.state[a[1]]["step"]) == 1

@@ -82,3 +82,65 @@ def test_load_state_dict_keeps_the_kernels_counter_words():
     opt._tickets["here"] = word
     opt.load_state_dict(optim.AdamW([_p(3)]).state_dict())
     assert opt._tickets["here"] is word
+
+
+def _with_state(lr=1e-3, n=4, bits=32):
+    """An optimiser on the CPU with a state written by hand, as a step on the GPU would have left it."""
+    p = _p(n)
+    opt = optim.AdamW([p], lr=lr, state_bits=bits, min_8bit_size=1)
+    opt._init_state(p, opt.param_groups[0])
+    for k, v in opt.state[p].items():
+        v.copy_(torch.arange(v.numel()).view(v.shape) + 1)
+    return opt, p
+
+
+@pytest.fixture
+def not_capturing(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+def test_load_state_dict_keeps_the_memory_of_rates_and_states(not_capturing):
+    rate = torch.tensor(1e-3)
+    opt, p = _with_state(rate)
+    other, q = _with_state(torch.tensor(5e-4))
+    held = dict(opt.state[p])
+    opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] is rate and float(rate) == float(torch.tensor(5e-4))
+    assert all(opt.state[p][k] is held[k] for k in held) and other.param_groups[0]["lr"] is not rate
+    opt.load_state_dict(_with_state(0.25)[0].state_dict())             # a number fills the tensor
+    assert opt.param_groups[0]["lr"] is rate and float(rate) == 0.25
+    number, _ = _with_state(0.5)
+    number.load_state_dict(other.state_dict())                         # a tensor takes a number's place
+    assert float(number.param_groups[0]["lr"]) == float(torch.tensor(5e-4))
+
+
+def test_load_state_dict_after_a_capture(not_capturing):
+    """What the graph writes is not given back: a state that is not loaded starts anew where it is, one of another kind
+    is refused before anything changes."""
+    opt, p = _with_state()
+    held = dict(opt.state[p])
+    opt._captured = True
+    eight, _ = _with_state(bits=8, lr=0.5)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(eight.state_dict())
+    assert opt.param_groups[0]["lr"] == 1e-3 and opt.param_groups[0]["state_bits"] == 32
+    assert all(opt.state[p][k] is v and bool((v != 0).all()) for k, v in held.items())
+    opt.load_state_dict(optim.AdamW([_p(4)]).state_dict())
+    assert all(opt.state[p][k] is v and bool((v == 0).all()) for k, v in held.items())
+    free, q = _with_state()                                            # nothing captured: as the base class
+    free.load_state_dict(eight.state_dict())
+    assert "exp_rms" in free.state[q]
+    free.load_state_dict(optim.AdamW([_p(4)]).state_dict())
+    assert not free.state[q]
+
+
+def test_groups_that_share_a_tensor_rate_load_one_rate(not_capturing):
+    def two(a, b):
+        return optim.AdamW([{"params": [_p(3)], "lr": a}, {"params": [_p(4)], "lr": b}])
+    rate = torch.tensor(1e-3)
+    opt = two(rate, rate)
+    opt.load_state_dict(two(0.5, 0.5).state_dict())
+    assert float(rate) == 0.5
+    with pytest.raises(ValueError):
+        opt.load_state_dict(two(0.5, 0.25).state_dict())
+    assert float(rate) == 0.5 and all(g["lr"] is rate for g in opt.param_groups)
