@@ -911,7 +911,8 @@ static Plan plan(int kind, int64_t M, int64_t N, int64_t K, bool direct)
     double least = 1e300;
     for (int i = 0; i < sizes; ++i) {
         const Tile& t = set[i];
-        const double tiles = (double)((M + t.bm - 1) / t.bm) * (double)((N + t.bn - 1) / t.bn);
+        const double tiles_n = N > 0 ? (double)((N + t.bn - 1) / t.bn) : 1.0;     // (N = 0: column sums alone)
+        const double tiles = (double)((M + t.bm - 1) / t.bm) * tiles_n;
         for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits / 2) {
             const int64_t per = k_tiles > 0 ? (k_tiles + splits - 1) / splits : 1;
             if (splits > 1 && per < 4) break;

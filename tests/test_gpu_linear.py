@@ -313,3 +313,18 @@ def test_modules_are_drop_ins(dev):
     got.sum().backward()
     for p, q in zip(plain.parameters(), net.parameters()):
         assert float((p.grad - q.grad.double()).abs().max()) <= 2000 * U * (1 + float(p.grad.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M", [1, 33, 65, 1000, 70001])
+def test_bias_gradient_without_input_features(dev, M, dtype):
+    """dy is small whole numbers, at most 4: sums up to 2^18 < 2^24 are exact in fp32 in any order and rounded once
+    (in fp16 to infinity from 65520 on, which 2 M does not reach: dy averages to 0)."""
+    for act in ("none", "relu"):
+        for N in (1, 5, 72):
+            dy = torch.randint(-4, 5, (M, N), generator=torch.Generator().manual_seed(M + N)).to(dtype)
+            b = torch.ones(N, dtype=dtype, device=dev, requires_grad=True)
+            y = _F().linear_act(torch.empty(M, 0, dtype=dtype, device=dev), torch.empty(N, 0, dtype=dtype, device=dev), b, act)
+            assert torch.equal(y, torch.ones(M, N, dtype=dtype, device=dev))
+            (db,) = torch.autograd.grad(y, [b], dy.to(dev))
+            assert torch.equal(db.cpu(), dy.double().sum(0).float().to(dtype))

@@ -90,3 +90,12 @@ def test_launches_of_too_many_threads_are_refused():
                                       i64(1), None, ctypes.c_size_t(0), None) == -2
         assert L.smlvm_linear_bwd(one, i64(1), None, i32(0), one, i64(1), one, i64(1), one, None, None, i32(kind), i32(0),
                                   i64(most), i64(1), i64(1), None, ctypes.c_size_t(0), None) == -2
+
+
+def test_bias_gradient_of_no_input_features_covers_every_row():
+    """K = 0 and no activation: db alone is a column sum over all M rows, split like any long sum (a plan that stops after
+    its first rows needs no workspace)."""
+    L = _native.lib()
+    for kind in (0, 1, 2):
+        with_inputs = L.smlvm_linear_bwd_workspace_bytes(kind, 0, 1 << 20, 5, 8)
+        assert with_inputs > 0 and L.smlvm_linear_bwd_workspace_bytes(kind, 0, 1 << 20, 5, 0) > 0
