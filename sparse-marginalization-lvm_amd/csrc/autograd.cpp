@@ -336,6 +336,12 @@ bool adamw_step(const pybind11::list& params, const pybind11::list& grads, const
 {
     struct Launch { at::Device device; at::ScalarType p, g; int32_t bits; std::vector<smlvm_adamw_tensor> table; };
     const at::NoGradGuard no_grad;
+    const bool rate_tensor = THPVariable_Check(lr.ptr());
+    if (rate_tensor) {                                // (the kernel reads it as one float)
+        const Tensor& rate = THPVariable_Unpack(lr.ptr());
+        TORCH_CHECK_TYPE(rate.scalar_type() == at::kFloat, "AdamW: a tensor lr must be float32, got ", rate.scalar_type());
+        TORCH_CHECK_VALUE(rate.numel() == 1, "AdamW: a tensor lr must have one element, got ", rate.sizes());
+    }
     std::vector<Launch> launches;
     std::vector<Tensor> keep;                         // alive until the launch: updated parameters and relaid gradients
     const size_t count = params.size();
@@ -386,25 +392,25 @@ bool adamw_step(const pybind11::list& params, const pybind11::list& grads, const
                              pybind11::cast<uint64_t>(numbers[i])});
         keep.push_back(p);
     }
-    const bool rate_tensor = THPVariable_Check(lr.ptr());
     bool captured = false;
     for (const Launch& l : launches) {
         const c10::DeviceGuard guard(l.device);
+        const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(l.device.index());
+        uint64_t capture = 0;
+        check(smlvm_stream_capture_id(stream.stream(), &capture), "smlvm_stream_capture_id");
         Tensor rate;
         double number = 0.0;
         if (rate_tensor) {
             rate = THPVariable_Unpack(lr.ptr());
             if (rate.device() != l.device) {
                 TORCH_CHECK_VALUE(!rate.is_cuda(), "AdamW: a tensor lr must be on the parameters' device");
+                TORCH_CHECK(!capture, "AdamW: a captured step reads a tensor lr at every replay: it must be on the parameters' device");
                 number = rate.item<double>();
                 rate = Tensor();
             }
         } else {
             number = pybind11::cast<double>(lr);
         }
-        const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(l.device.index());
-        uint64_t capture = 0;
-        check(smlvm_stream_capture_id(stream.stream(), &capture), "smlvm_stream_capture_id");
         captured |= capture != 0;
         Tensor ticket;                                // (a word per stream: steps on two of them may overlap)
         if (!capture) {

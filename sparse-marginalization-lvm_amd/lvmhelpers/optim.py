@@ -32,7 +32,7 @@ class AdamW(torch.optim.Optimizer):
     params: float32, float16 or bfloat16 GPU tensors (dense, any memory order); a 16-bit weight is
         updated in fp32 and rounded to nearest.
     lr: a number, or a float32 tensor of one element on the parameters' device, which a captured
-        step then reads at every replay.
+        step then reads at every replay (one on the CPU is read when a step is called, and refused in a capture).
     state_bits: 32, or 8 for parameters of at least `min_8bit_size` elements (smaller ones -- biases,
         norms -- keep 32 bits).  The choice is made when a parameter's state is first created.
     seed: of the 8-bit states' rounding.

@@ -509,3 +509,19 @@ def test_a_captured_step_goes_on_after_load_state_dict(dev, bits):
     graph.replay()
     opt_f.step(grads=grads)
     assert all(torch.equal(p, f) for p, f in zip(a, fresh)) and int(opt_a.state[a[1]]["step"]) == 1
+
+
+def test_a_rate_on_the_cpu_is_not_captured(dev):
+    """A replay could not see it change."""
+    p, g = _param((300,), torch.float32, dev, 1), _grad((300,), torch.float32, dev, 2)
+    opt = _optim().AdamW([p], lr=torch.tensor(1e-2))
+    opt.step(grads=[g])                            # eagerly it is read at the call
+    other = p.clone()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="tensor lr"):
+        with torch.cuda.graph(graph):
+            opt.step(grads=[g])
+    torch.cuda.synchronize()
+    assert torch.equal(p, other) and int(opt.state[p]["step"]) == 1
+    opt.step(grads=[g])
+    assert int(opt.state[p]["step"]) == 2

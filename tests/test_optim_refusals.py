@@ -144,3 +144,17 @@ def test_groups_that_share_a_tensor_rate_load_one_rate(not_capturing):
     with pytest.raises(ValueError):
         opt.load_state_dict(two(0.5, 0.25).state_dict())
     assert float(rate) == 0.5 and all(g["lr"] is rate for g in opt.param_groups)
+
+
+@pytest.mark.parametrize("rate,error", [(torch.tensor(1e-3, dtype=torch.float64), TypeError), (torch.tensor(1e-3).bfloat16(), TypeError),
+                                        (torch.tensor(1), TypeError), (torch.full((2,), 1e-3), ValueError),
+                                        (torch.empty(0), ValueError)])
+def test_a_tensor_rate_is_checked_at_every_step(rate, error):
+    """One that took the place of the first rate, by hand or from a checkpoint."""
+    opt = optim.AdamW([_p(3)], lr=1e-3)
+    opt.step()                                     # (no gradients: nothing to do)
+    opt.param_groups[0]["lr"] = rate
+    with pytest.raises(error):
+        opt.step()
+    opt.param_groups[0]["lr"] = torch.tensor([1e-3])
+    opt.step()
