@@ -444,7 +444,7 @@ int smlvm_policy_loss(const void* logits, int32_t kind, int64_t stride_b, int64_
  * cores to fp32's accuracy (products below 2^-23 |x||w| are left out); an infinite operand then gives
  * NaN where fp32 might give an infinity.
  * bias, residual nullable.  pre (nullable) [M, N]: act's argument, which the backward needs; fp32, next to bf16 tensors fp16
- * (held within its range).
+ * (held within its range; for relu, positive numbers stay positive).
  * workspaces: smlvm_linear_fwd_workspace_bytes / _bwd_workspace_bytes bytes, 16-byte aligned, contents ignored. */
 size_t smlvm_linear_fwd_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K);
 size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, int64_t M, int64_t N, int64_t K);

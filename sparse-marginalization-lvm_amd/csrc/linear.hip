@@ -173,15 +173,20 @@ __device__ __forceinline__ void store8(T* p, int have, const float (&x)[8])
 // act's argument for the backward: fp32, next to bf16 tensors fp16.  The slope is taken from it, and its rounding must
 // not add to that of dh and of the gradient itself (two roundings, 1.41 times one): with bf16 the gradients of bf16
 // tensors were 1.6 times one rounding off, with fp16 those of fp16 tensors 1.52 times; with 3 bits more (fp16
-// next to bf16) and with fp32 1.42.  Beyond fp16's range every activation's slope is constant.
+// next to bf16) and with fp32 1.42.  Beyond fp16's range every activation's slope is constant; below it every one
+// is continuous but relu's, whose positive arguments stay positive.
 template <class T> struct PreOf { typedef float type; };
 template <> struct PreOf<bf16_t> { typedef f16_t type; };
 template <class T>
-__device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const float (&x)[8])
+__device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const float (&x)[8], int act)
 {
     float h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = sizeof(typename PreOf<T>::type) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    if (sizeof(typename PreOf<T>::type) == 2 && act == kRelu) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = h[j] > 0.0f ? fmaxf(h[j], 0x1p-24f) : h[j];
+    }
     store8(static_cast<typename PreOf<T>::type*>(pre) + at, have, h);
 }
 
@@ -193,7 +198,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& g, int64_t m, int64_t n,
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += b[j];
     }
-    if (g.pre) store_pre<T>(g.pre, m * g.N + n, have, x);
+    if (g.pre) store_pre<T>(g.pre, m * g.N + n, have, x, g.act);
     act_all<sizeof(T) == 2>(g.act, x);
     if (g.res) {
 #pragma unroll

@@ -328,3 +328,40 @@ def test_bias_gradient_without_input_features(dev, M, dtype):
             assert torch.equal(y, torch.ones(M, N, dtype=dtype, device=dev))
             (db,) = torch.autograd.grad(y, [b], dy.to(dev))
             assert torch.equal(db.cpu(), dy.double().sum(0).float().to(dtype))
+
+
+def _check_tiny_relu(dev, dtype, M, N, K, res):
+    """h is a single product, some 2^-27 (below half of fp16's smallest number) of either sign: its slope is 0 or 1.  dy is
+    small whole numbers, so db is exact up to its rounding; dx and dw as in _check, dh being exact."""
+    g = torch.Generator().manual_seed(M + N)
+
+    def sized(shape, low):                          # +- [1, 1.4) low
+        return ((1 + 0.4 * torch.rand(shape, generator=g)) * low * (1 - 2 * torch.randint(0, 2, shape, generator=g))).to(dtype)
+    x = torch.zeros(M, K, dtype=dtype)
+    at = torch.randint(0, K, (M,), generator=g)
+    x[torch.arange(M), at] = sized((M,), 2.0 ** -13)
+    w, dy = sized((N, K), 2.0 ** -14), torch.randint(-4, 5, (M, N), generator=g).to(dtype)
+    b = torch.zeros(N, dtype=dtype)
+    r = torch.randn(M, N, generator=g).to(dtype) if res else None
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b)]
+    y = _F().linear_act(*leaves, "relu", None if r is None else r.to(dev))
+    X, W, DY = (t.double().to(dev) for t in (x, w, dy))
+    h = X @ W.t().contiguous()
+    assert float(h.abs().max()) < 2.0 ** -25 and float(h.abs().min()) > 2.0 ** -28
+    want = h.clamp_min(0) + (0 if r is None else r.double().to(dev))
+    _within(y.detach(), want.cpu(), (_half(dtype) * 1.01 * want.abs() + 2.0 ** -25).cpu())
+    dh = DY * (h > 0)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.to(dev))
+    assert torch.equal(db.cpu(), dh.sum(0).to(dtype).cpu())
+    _within(dx, (dh @ W).cpu(), (_sum_err(N, dtype) * (dh.abs() @ W.abs()) + _half(dtype) * 1.01 * (dh @ W).abs() + 2.0 ** -25 * (dtype == torch.float16)).cpu())
+    dht = dh.t().contiguous()
+    _within(dw, (dht @ X).cpu(), (_sum_err(M, dtype) * (dht.abs() @ X.abs()) + _half(dtype) * 1.01 * (dht @ X).abs() + 2.0 ** -25 * (dtype == torch.float16)).cpu())
+
+
+TINY = [(3, 40, 16), (70, 97, 47), (128, 256, 64), (6, 64, 40000)]      # few rows, unaligned, aligned, split over k
+
+
+@pytest.mark.parametrize("M,N,K", TINY)
+def test_relu_with_a_residual_keeps_the_sign_of_tiny_arguments(dev, M, N, K):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        _check_tiny_relu(dev, dtype, M, N, K, True)
