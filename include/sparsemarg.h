@@ -443,8 +443,8 @@ int smlvm_policy_loss(const void* logits, int32_t kind, int64_t stride_b, int64_
  * once.  fp32 operands are split into bf16 parts without loss and multiplied on the bf16 matrix
  * cores to fp32's accuracy (products below 2^-23 |x||w| are left out); an infinite operand then gives
  * NaN where fp32 might give an infinity.
- * bias, residual nullable.  pre (nullable) [M, N]: act's argument, which the backward needs; fp32, next to bf16 tensors fp16
- * (held within its range; for relu, positive numbers stay positive).
+ * bias, residual nullable.  pre (nullable) [M, N]: act's argument, which the backward needs; fp32, but next to bf16 tensors,
+ * and for relu next to fp16 ones, fp16 (held within its range; for relu, positive numbers stay positive).
  * workspaces: smlvm_linear_fwd_workspace_bytes / _bwd_workspace_bytes bytes, 16-byte aligned, contents ignored. */
 size_t smlvm_linear_fwd_workspace_bytes(int32_t kind, int64_t M, int64_t N, int64_t K);
 size_t smlvm_linear_bwd_workspace_bytes(int32_t kind, int32_t act, int64_t M, int64_t N, int64_t K);
@@ -452,7 +452,8 @@ int smlvm_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, con
                      const void* residual, int64_t ldr, void* y, void* pre, int32_t kind, int32_t act,
                      int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 /* With dh = dy act'(h):  dx[m][k] = sum_n dh[m][n] w[n][k];  dw[n][k] = sum_m dh[m][n] x[m][k];  db[n] = sum_m dh[m][n].
- * h [M, N] is `pre`, or with h_is_y != 0 (relu without a residual only) y; unused for act 0.  dh is rounded to
+ * h [M, N] is `pre`, or with h_is_y != 0 (relu without a residual only) y, whose sign is the argument's but where y
+ * was rounded to 0 (fp16: 0 < h < 2^-25); unused for act 0.  dh is rounded to
  * `kind`.  dx, dw, db nullable (db only with dw).  Rows of dy start ldy elements apart (= N unless act is 0). */
 int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int32_t h_is_y, const void* x, int64_t ldx,
                      const void* w, int64_t ldw, void* dx, void* dw, void* db, int32_t kind, int32_t act, int64_t M,

@@ -82,6 +82,9 @@ struct Rows {
 
 enum { kRelu = 1 };
 
+// relu's slope can be told from its result, but for fp16's: arguments below 2^-25 have the result 0 there.
+bool sign_of_y(int64_t act, int32_t kind, bool residual) { return act == kRelu && !residual && kind != SMLVM_F16; }
+
 Tensor linear_forward(const Tensor& x_, const Tensor& w_, const Maybe& b, const Maybe& r_, int64_t act, Tensor* pre)
 {
     const c10::DeviceGuard guard(x_.device());
@@ -91,7 +94,7 @@ Tensor linear_forward(const Tensor& x_, const Tensor& w_, const Maybe& b, const 
     std::optional<Rows> r;
     if (r_) r.emplace(*r_);
     Tensor y = at::empty({M, N}, x_.options());
-    if (pre) *pre = at::empty({M, N}, x_.options().dtype(kind == SMLVM_BF16 ? at::kHalf : at::kFloat));
+    if (pre) *pre = at::empty({M, N}, x_.options().dtype(kind == SMLVM_F32 || (kind == SMLVM_F16 && act != kRelu) ? at::kFloat : at::kHalf));
     const size_t bytes = smlvm_linear_fwd_workspace_bytes(kind, M, N, K);
     const Tensor ws = workspace(bytes, x_);
     check(smlvm_linear_fwd(ptr(x.t), x.ld, ptr(w.t), w.ld, ptr(b), r ? ptr(r->t) : nullptr, r ? r->ld : N, ptr(y),
@@ -100,12 +103,12 @@ Tensor linear_forward(const Tensor& x_, const Tensor& w_, const Maybe& b, const 
     return y;
 }
 
-// act(x w^T + b) + r.  For the backward the forward leaves act's argument (float32, or float16 next to bfloat16
-// tensors; relu without a residual keeps its output instead: y > 0 exactly where its argument is).
+// act(x w^T + b) + r.  For the backward the forward leaves act's argument (include/sparsemarg.h says in which type), or
+// relu's result in its place.
 struct LinearAct : Function<LinearAct> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act)
     {
-        const bool need = wants(x) || wants(w) || wants(b), own_sign = act == kRelu && !r;
+        const bool need = wants(x) || wants(w) || wants(b), own_sign = sign_of_y(act, kind_of(x), r.has_value());
         Tensor pre;
         Tensor y = linear_forward(x, w, b, r, act, need && act && !own_sign ? &pre : nullptr);
         ctx->saved_data["act"] = act;
@@ -133,7 +136,7 @@ struct LinearAct : Function<LinearAct> {
             if (want_db) db = at::empty({N}, x_.options());
             const size_t bytes = smlvm_linear_bwd_workspace_bytes(kind, (int32_t)act, M, N, K);
             const Tensor ws = workspace(bytes, x_);
-            check(smlvm_linear_bwd(ptr(dy.t), dy.ld, act ? ptr(saved[2]) : nullptr, act == kRelu && !has_r, ptr(x.t), x.ld, ptr(w.t),
+            check(smlvm_linear_bwd(ptr(dy.t), dy.ld, act ? ptr(saved[2]) : nullptr, sign_of_y(act, kind, has_r), ptr(x.t), x.ld, ptr(w.t),
                                    w.ld, ptr(dx), ptr(dw), ptr(db), kind, (int32_t)act, M, N, K, ptr(ws), bytes, stream_of(x_)),
                   "smlvm_linear_bwd");
             if (!want_dw) dw = Tensor();

@@ -175,19 +175,23 @@ __device__ __forceinline__ void store8(T* p, int have, const float (&x)[8])
 // tensors were 1.6 times one rounding off, with fp16 those of fp16 tensors 1.52 times; with 3 bits more (fp16
 // next to bf16) and with fp32 1.42.  Beyond fp16's range every activation's slope is constant; below it every one
 // is continuous but relu's, whose positive arguments stay positive.
-template <class T> struct PreOf { typedef float type; };
-template <> struct PreOf<bf16_t> { typedef f16_t type; };
+// Of relu's argument only the sign is read: fp16 next to fp16, too.
 template <class T>
 __device__ __forceinline__ void store_pre(void* pre, int64_t at, int have, const float (&x)[8], int act)
 {
+    const bool relu = act == kRelu;
+    if (sizeof(T) == 4 || (KindOf<T>::value == SMLVM_F16 && !relu)) {
+        store8(static_cast<float*>(pre) + at, have, x);
+        return;
+    }
     float h[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = sizeof(typename PreOf<T>::type) == 4 || x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
-    if (sizeof(typename PreOf<T>::type) == 2 && act == kRelu) {
+    for (int j = 0; j < 8; ++j) h[j] = x[j] != x[j] ? x[j] : fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+    if (relu) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = h[j] > 0.0f ? fmaxf(h[j], 0x1p-24f) : h[j];
     }
-    store8(static_cast<typename PreOf<T>::type*>(pre) + at, have, h);
+    store8(static_cast<f16_t*>(pre) + at, have, h);
 }
 
 // 8 consecutive n of row m: bias, activation, residual, stores
@@ -1177,7 +1181,7 @@ extern "C" int smlvm_linear_bwd(const void* dy, int64_t ldy, const void* h, int3
 #define ACT_BWD(T, H) hipLaunchKernelGGL((act_bwd_kernel<T, H>), grid, dim3(256), 0, stream, static_cast<const T*>(dy), \
                                          static_cast<const H*>(h), reinterpret_cast<T*>(ws), M, N, act, p.groups, p.rows, part)
         if (kind == SMLVM_F32) ACT_BWD(float, float);
-        else if (kind == SMLVM_F16 && h_is_y) ACT_BWD(f16_t, f16_t);
+        else if (kind == SMLVM_F16 && act == kRelu) ACT_BWD(f16_t, f16_t);             // (y or pre)
         else if (kind == SMLVM_F16) ACT_BWD(f16_t, float);
         else if (h_is_y) ACT_BWD(bf16_t, bf16_t);
         else ACT_BWD(bf16_t, f16_t);

@@ -365,3 +365,10 @@ TINY = [(3, 40, 16), (70, 97, 47), (128, 256, 64), (6, 64, 40000)]      # few ro
 def test_relu_with_a_residual_keeps_the_sign_of_tiny_arguments(dev, M, N, K):
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         _check_tiny_relu(dev, dtype, M, N, K, True)
+
+
+@pytest.mark.parametrize("M,N,K", TINY)
+def test_relu_without_a_residual_keeps_the_sign_of_tiny_arguments(dev, M, N, K):
+    """(the sign of y would not do in fp16, where these results are 0)"""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        _check_tiny_relu(dev, dtype, M, N, K, False)
