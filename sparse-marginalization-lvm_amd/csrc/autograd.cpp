@@ -45,6 +45,15 @@ void* ptr(const Maybe& t) { return t ? ptr(*t) : nullptr; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const Maybe& t) { return t && wants(*t); }
 
+// Forward-mode derivatives: a dual tensor need not require a gradient, and its tangent would be lost without a word.
+void no_tangent(const Tensor& t)
+{
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+        C10_THROW_ERROR(NotImplementedError, "this operator has no forward-mode derivative");
+}
+void no_tangent(const Maybe& t) { if (t) no_tangent(*t); }
+template <class... Ts> void no_tangents(const Ts&... t) { (no_tangent(t), ...); }
+
 Tensor workspace(size_t bytes, const Tensor& like)
 {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
@@ -150,6 +159,7 @@ struct LinearAct : Function<LinearAct> {
 
 Tensor linear_act(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act)
 {
+    no_tangents(x, w, b, r);
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearAct::apply(x, w, b, r, act);
     return linear_forward(x, w, b, r, act, nullptr);
 }
@@ -218,6 +228,7 @@ struct TokenLogprobs : Function<TokenLogprobs> {
 
 std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& actions, const Maybe& mask)
 {
+    no_tangents(logits);
     const bool record = at::GradMode::is_enabled() && wants(logits);
     variable_list out = record ? TokenLogprobs::apply(logits, actions, mask) : logprobs_forward(logits, actions, mask, false);
     return {out[0], out[1]};
@@ -301,6 +312,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> clipped_policy_loss(
     const Tensor& logits, const Tensor& actions, const Tensor& old_logp, const Tensor& advantages, const Maybe& ref_logp,
     const Maybe& mask, double clip_low, double clip_high, double kl_coeff, double entropy_coeff, bool mean)
 {
+    no_tangents(logits, old_logp, advantages, ref_logp);
     const auto out = ClippedPolicyLoss::apply(at::GradMode::is_enabled() ? logits : logits.detach(), actions, old_logp, advantages,
                                               ref_logp, mask, clip_low, clip_high, kl_coeff, entropy_coeff, mean);
     return {out[0], out[1], out[2], out[3], out[4]};

@@ -372,3 +372,20 @@ def test_relu_without_a_residual_keeps_the_sign_of_tiny_arguments(dev, M, N, K):
     """(the sign of y would not do in fp16, where these results are 0)"""
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         _check_tiny_relu(dev, dtype, M, N, K, False)
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    """Through every public way in; a tensor of the level without a tangent is an ordinary one."""
+    import torch.autograd.forward_ad as fwad
+    from lvmhelpers import fused
+    F_ = _F()
+    x, w, z = torch.randn(3, 4, device=dev), torch.randn(5, 4, device=dev), torch.randn(2, 3, device=dev)
+    a, v = torch.zeros(2, dtype=torch.int64, device=dev), torch.zeros(2, device=dev)
+    base, layer = F_.linear_act(x, w), fused.LinearAct(4, 5).to(dev)
+    with fwad.dual_level():
+        dual, dz = fwad.make_dual(x, torch.ones_like(x)), fwad.make_dual(z, torch.ones_like(z))
+        for call in (lambda: F_.linear_act(dual, w), lambda: F_.linear_act(dual.view(1, 3, 4), w), lambda: layer(dual),
+                     lambda: F_.linear_act(w, dual), lambda: F_.token_logprobs(dz, a), lambda: F_.clipped_policy_loss(dz, a, v, v)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(F_.linear_act(x, w), base)
