@@ -29,8 +29,8 @@ class AdamW(torch.optim.Optimizer):
     """p <- p (1 - lr wd) - lr m^ / (sqrt(v^) + eps), m^ and v^ the bias-corrected averages of the
     gradient and its square (torch.optim.AdamW's update).
 
-    params: float32, float16 or bfloat16 GPU tensors (dense, any memory order); a 16-bit weight is
-        updated in fp32 and rounded to nearest.
+    params: float32, float16 or bfloat16 GPU tensors (dense, any memory order, no two of them sharing
+        memory); a 16-bit weight is updated in fp32 and rounded to nearest.
     lr: a number, or a float32 tensor of one element on the parameters' device, which a captured
         step then reads at every replay (one on the CPU is read when a step is called, and refused in a capture).
     state_bits: 32, or 8 for parameters of at least `min_8bit_size` elements (smaller ones -- biases,
@@ -81,6 +81,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: eps and weight_decay must not be negative")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 32 or 8, got {group['state_bits']}")
+        if len(set(map(id, group["params"]))) != len(group["params"]):
+            raise ValueError("AdamW: a parameter may be in a group only once")
         for p in group["params"]:
             if p.dtype not in _FLOATS:
                 raise TypeError(f"AdamW: parameters are float32, float16 or bfloat16, got {p.dtype}")

@@ -158,3 +158,15 @@ def test_a_tensor_rate_is_checked_at_every_step(rate, error):
         opt.step()
     opt.param_groups[0]["lr"] = torch.tensor([1e-3])
     opt.step()
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains")
+def test_a_parameter_twice_in_a_group_is_refused():
+    """Two entries of one launch would update the same memory at the same time (torch only warns)."""
+    p = _p(3)
+    with pytest.raises(ValueError):
+        optim.AdamW([p, _p(4), p])
+    opt = optim.AdamW([_p(4)])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [p, p]})
+    assert len(opt.param_groups) == 1
