@@ -441,7 +441,7 @@ int smlvm_policy_loss(const void* logits, int32_t kind, int64_t stride_b, int64_
  * Rows of x, w, residual start ldx, ldw, ldr elements apart (elements within a row consecutive); y,
  * pre, dy, dh, dx, dw contiguous unless a stride is given.  Sums in fp32; 16-bit results are rounded
  * once.  fp32 operands are split into bf16 parts without loss and multiplied on the bf16 matrix
- * cores to fp32's accuracy (products below 2^-23 |x||w| are left out); an infinite operand then gives
+ * cores to fp32's accuracy (2^-22 |x||w| at most is left out of a product); an infinite operand then gives
  * NaN where fp32 might give an infinity.
  * bias, residual nullable.  pre (nullable) [M, N]: act's argument, which the backward needs; fp32, but next to bf16 tensors,
  * and for relu next to fp16 ones, fp16 (held within its range; for relu, positive numbers stay positive).

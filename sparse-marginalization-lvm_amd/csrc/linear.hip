@@ -12,9 +12,10 @@
 //
 // 16-bit operands go from memory to LDS directly (buffer_load_dwordx4 ... lds) where rows are aligned to 16
 // bytes, else through registers.  fp32 operands are split exactly into three bf16 parts of 8 bits,
-// x = x1 + x2 + x3 (truncation leaves a remainder of the same sign, 24 bits in all), and the six
-// products of order >= 2^-16 are summed in fp32 on the bf16 matrix cores: what is left out is
-// below 2^-23 of |x||w| per term, the size of fp32's own rounding.  Six bf16 products at 2.5 PFLOP/s
+// x = x1 + x2 + x3: x1 is x cut off (rounded, the largest numbers would become infinities), x2 the remainder rounded
+// to nearest, and what that leaves has 8 bits.  With |x2| <= 2^-7 |x| and |x3| <= 2^-16 |x| the six products of
+// order >= 2^-16 are summed in fp32 on the bf16 matrix cores; x2 w3 + x3 w2 + x3 w3 is left out, 2^-22 |x||w| at most
+// and of either sign (with x2 cut off, too, it was twice that and always the product's).  Six bf16 products at 2.5 PFLOP/s
 // are 0.42 PFLOP/s, against 0.157 of the fp32 matrix instructions.
 //
 // Measured, [8192 x 4096] [8192 x 4096]^T bf16 with gelu and a residual: forward 530 us (425 the main loop, 1.29
@@ -25,7 +26,9 @@
 
 namespace smlvm {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -431,17 +434,15 @@ struct Through {
                 u32x4 plane[3];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {                            // two elements -> one word of each plane
-                    uint32_t x[2] = {held[i][j >> 1][(j & 1) * 2], held[i][j >> 1][(j & 1) * 2 + 1]};
+                    float x[2];
+                    const uint32_t raw[2] = {held[i][j >> 1][(j & 1) * 2], held[i][j >> 1][(j & 1) * 2 + 1]};
+                    plane[0][j] = __builtin_amdgcn_perm(raw[1], raw[0], 0x07060302);   // high halves
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        plane[q][j] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302);   // high halves
-                        if (q < 2) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                x[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, x[e]) -
-                                                                        __builtin_bit_cast(float, x[e] & 0xFFFF0000u));
-                        }
-                    }
+                    for (int e = 0; e < 2; ++e) x[e] = __builtin_bit_cast(float, raw[e]) - __builtin_bit_cast(float, raw[e] & 0xFFFF0000u);
+                    plane[1][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[0], x[1]}), bf16x2));
+                    x[0] -= __builtin_bit_cast(float, plane[1][j] << 16);
+                    x[1] -= __builtin_bit_cast(float, plane[1][j] & 0xFFFF0000u);
+                    plane[2][j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[1]), __builtin_bit_cast(uint32_t, x[0]), 0x07060302);
                 }
 #pragma unroll
                 for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(to + q * Tl::kBytes) = plane[q];

@@ -389,3 +389,21 @@ def test_forward_mode_derivatives_are_refused(dev):
             with pytest.raises(NotImplementedError):
                 call()
         assert torch.equal(F_.linear_act(x, w), base)
+
+
+def test_fp32_products_one_by_one(dev):
+    """Single products of any operands, the worst ones of a split in three parts among them (both far from their first
+    part's 8 bits).  Left out: 2^-22 |x||w|; rounded: the last sum by u, those before it, of 2^-6 |x||w|
+    and less, by less than u in all -- 6 u."""
+    g = torch.Generator().manual_seed(0)
+    worst = torch.tensor([1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -7 - 2.0 ** -16, 1 + 2.0 ** -7 - 2.0 ** -15 + 2.0 ** -16 - 2.0 ** -23,
+                          1 + 2.0 ** -8 + 2.0 ** -16 - 2.0 ** -23, 1 + 2.0 ** -8, 1 + 2.0 ** -8 - 2.0 ** -23, 2 - 2.0 ** -23, 1.0])
+    worst = torch.cat([worst, -worst])
+    for M, N in ((64, 64), (256, 512)):
+        x, w = 1 + torch.rand(M, generator=g), 1 + torch.rand(N, generator=g)
+        x[:16], w[:16] = worst, worst
+        x, w = (t * torch.exp2(torch.randint(-30, 31, t.shape, generator=g).float()) for t in (x, w))
+        wide = torch.zeros(N, M)                       # row n holds w_n in every column: y[m][n] = x_m w_n
+        wide[:] = w[:, None]
+        want = x.double()[:, None] * w.double()[None, :]
+        _within(F_one(torch.diag(x).to(dev), wide.to(dev)), want, 6 * U * want.abs())
