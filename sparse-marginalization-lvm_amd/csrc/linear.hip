@@ -48,12 +48,13 @@ template <bool FAST>
 __device__ __forceinline__ float sigmoid_f(float h)
 {
     if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * h));
-    // fp32: e^-h = 2^y (1 + ln2 d) with y + d = -h log2 e to 48 bits; off by 6 half steps at most (2 from v_exp, 2 from
-    // v_rcp, one each from the sums), in a third of the instructions of expf and a division ([42803 x 16] [6336 x 16]^T
-    // with silu and a residual: 945 -> 800 us).  Beyond 88 the result is 0 or 1 to fp32.
-    const float g = fminf(fmaxf(h, -88.0f), 88.0f), y = -1.44269504f * g;
+    // fp32: e^-h = 2^y (1 + ln2 d) with y + d = -h log2 e to 48 bits; off by 7 half steps at most (2 from v_exp, 2 from
+    // v_rcp, one each from the sums and the product), in a third of the instructions of expf and a division
+    // ([42803 x 16] [6336 x 16]^T with silu and a residual: 945 -> 800 us).  From -89 on 2^y is infinite and the result
+    // 0: not 1 / (1 + e^88), which times -3e38 is -2 (the clamp keeps d finite).
+    const float g = fminf(fmaxf(h, -104.0f), 104.0f), y = -1.44269504f * g;
     const float d = fmaf(-g, 1.44269504f, -y) + g * -1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(y), s = __builtin_amdgcn_rcpf(1.0f + fmaf(e, 0.693147181f * d, e));
+    const float e = __builtin_amdgcn_exp2f(y) * fmaf(0.693147181f, d, 1.0f), s = __builtin_amdgcn_rcpf(1.0f + e);
     return h != h ? h : s;
 }
 // the normal distribution function

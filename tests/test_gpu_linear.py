@@ -407,3 +407,36 @@ def test_fp32_products_one_by_one(dev):
         wide[:] = w[:, None]
         want = x.double()[:, None] * w.double()[None, :]
         _within(F_one(torch.diag(x).to(dev), wide.to(dev)), want, 6 * U * want.abs())
+
+
+def _slope(name, h):
+    phi = 0.5 * torch.erfc(-h * 0.5 ** 0.5)
+    s = torch.sigmoid(h)
+    return {"none": torch.ones_like(h), "relu": (h > 0).double(), "gelu": phi + h * torch.exp(-0.5 * h * h) / (2 * torch.pi) ** 0.5,
+            "silu": s * (1 + h * torch.sigmoid(-h)), "sigmoid": s * torch.sigmoid(-h), "tanh": 1 / torch.cosh(h) ** 2}[name]
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_their_whole_range(dev, act, dtype):
+    """Arguments from 0 to the type's largest number, given as the bias (x is 0), so that they are exact; those of bf16 tensors
+    are exact in fp16 too, or beyond its range.  Result: 8 u (|a| + 1) and its rounding; slope, summed M times in
+    db: M times 12 u, each dh's rounding and the sum's own."""
+    big = [65504.0] if dtype == torch.float16 else [65280.0, 1e6, 1e30, 1e38, 3e38]
+    h = torch.tensor([0.0, 1e-3, 0.5, 1, 3, 5, 8, 12, 20, 30, 50, 80, 86, 87, 87.5, 88, 88.5, 89, 90, 100, 104, 105, 150, 1000, 1e4] + big)
+    h = h.to(dtype)
+    assert bool(h.isfinite().all())
+    h = torch.cat([h, -h])
+    if act == "relu":
+        h = h[h != 0]                                   # (the corner has no slope)
+    H, N, half = h.double(), h.numel(), _half(dtype)
+    for M in (3, 40):
+        b = h.to(dev).requires_grad_(True)
+        x, w = torch.zeros(M, 8, dtype=dtype, device=dev), torch.ones(N, 8, dtype=dtype, device=dev)
+        y = _F().linear_act(x, w, b, act)
+        a = 0.5 * H * torch.erfc(-H * 0.5 ** 0.5) if act == "gelu" else _act(act, H)
+        want = a.expand(M, N)
+        _within(y.detach(), want, 8 * U * (want.abs() + (act not in ("none", "relu"))) + 1.01 * half * want.abs() + 2.0 ** -25 * (dtype == torch.float16))
+        (db,) = torch.autograd.grad(y, [b], torch.ones(M, N, dtype=dtype, device=dev))
+        s = M * _slope(act, H)
+        _within(db, s, M * (12 * U * (act not in ("none", "relu")) + 2.0 ** -25 * (dtype == torch.float16)) + (2.02 * half + 60 * U) * s.abs())
