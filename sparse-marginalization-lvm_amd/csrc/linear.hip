@@ -75,7 +75,7 @@ __device__ __forceinline__ float phi_f(float h)
         const float half = 0.5f * t * __builtin_amdgcn_exp2f(fmaf(-z, z, p) * 1.44269504f);
         return h >= 0.0f ? 1.0f - half : half;
     } else {
-        return 0.5f * (1.0f + erff(h * 0.70710678118654752f));
+        return 0.5f * erfcf(h * -0.70710678118654752f);   // (1 + erf has no digits left below -5)
     }
 }
 

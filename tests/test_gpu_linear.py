@@ -440,3 +440,19 @@ def test_activations_over_their_whole_range(dev, act, dtype):
         (db,) = torch.autograd.grad(y, [b], torch.ones(M, N, dtype=dtype, device=dev))
         s = M * _slope(act, H)
         _within(db, s, M * (12 * U * (act not in ("none", "relu")) + 2.0 ** -25 * (dtype == torch.float16)) + (2.02 * half + 60 * U) * s.abs())
+
+
+def test_fp32_gelu_keeps_relative_accuracy_in_its_tail(dev):
+    """Phi(h) of h < 0 down to fp32's smallest normal numbers.  z = h / sqrt 2 and h^2 / 2 are rounded, which moves Phi and
+    e^(-h^2 / 2) by 2 z^2 u = h^2 u and a half of it, relative; erfc is good to 32 u, the rest to 8.  The slope is
+    Phi + h phi, each as good."""
+    h = -torch.linspace(0.5, 12.5, 2001)
+    H = h.double()
+    phi, pdf = 0.5 * torch.erfc(-H * 0.5 ** 0.5), torch.exp(-0.5 * H * H) / (2 * torch.pi) ** 0.5
+    rel = (2 * H * H + 40) * U
+    for M in (3, 40):
+        b = h.to(dev).requires_grad_(True)
+        y = _F().linear_act(torch.zeros(M, 8, device=dev), torch.ones(h.numel(), 8, device=dev), b, "gelu")
+        _within(y.detach(), (H * phi).expand(M, -1), (rel * (H * phi).abs()).expand(M, -1))
+        (db,) = torch.autograd.grad(y, [b], torch.ones_like(y))
+        _within(db, M * (phi + H * pdf), M * (rel + 40 * U) * (phi + (H * pdf).abs()))
