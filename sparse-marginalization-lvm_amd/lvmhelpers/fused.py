@@ -54,10 +54,10 @@ def fuse_linears(module):
     """Replaces, in place, every nn.Linear inside the nn.Sequentials of `module` (itself included) by a
     LinearAct with the same parameters, taking the activation module that follows it into the
     epilogue; that one's place holds an nn.Identity, so that state_dict keys do not change.  Linears with
-    hooks or of another type than float32, float16, bfloat16, subclasses of nn.Linear and of nn.Sequential, and
-    activations without an epilogue stay as they are.  Returns `module`."""
+    hooks, with a forward of their own or of another type than float32, float16, bfloat16, subclasses of nn.Linear and
+    of nn.Sequential, and activations without an epilogue stay as they are.  Returns `module`."""
     def hooked(m):
-        return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+        return "forward" in vars(m) or any(v for k, v in vars(m).items() if k.endswith("_hooks"))
 
     for seq in [m for m in module.modules() if type(m) is torch.nn.Sequential]:
         for i, lin in enumerate(seq):

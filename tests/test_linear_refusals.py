@@ -99,3 +99,18 @@ def test_bias_gradient_of_no_input_features_covers_every_row():
     for kind in (0, 1, 2):
         with_inputs = L.smlvm_linear_bwd_workspace_bytes(kind, 0, 1 << 20, 5, 8)
         assert with_inputs > 0 and L.smlvm_linear_bwd_workspace_bytes(kind, 0, 1 << 20, 5, 0) > 0
+
+
+def test_fuse_linears_leaves_instances_of_their_own():
+    """A forward put on the instance (as wrappers of modules do) and hooks on the state dict would be lost without a word."""
+    def linear():
+        return torch.nn.Linear(3, 3)
+    patched, saved, loaded, act = linear(), linear(), linear(), torch.nn.ReLU()
+    patched.forward = lambda x: x
+    saved.register_state_dict_post_hook(lambda *a: None)
+    loaded.register_load_state_dict_post_hook(lambda *a: None)
+    act.forward = lambda x: x
+    for m in (patched, saved, loaded):
+        assert fused.fuse_linears(torch.nn.Sequential(m))[0] is m
+    net = fused.fuse_linears(torch.nn.Sequential(linear(), act))
+    assert net[0].activation == "none" and net[1] is act
