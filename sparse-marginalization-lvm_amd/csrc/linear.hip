@@ -18,8 +18,8 @@
 // and of either sign (with x2 cut off, too, it was twice that and always the product's).  Six bf16 products at 2.5 PFLOP/s
 // are 0.42 PFLOP/s, against 0.157 of the fp32 matrix instructions.
 //
-// Measured, [8192 x 4096] [8192 x 4096]^T bf16 with gelu and a residual: forward 530 us (425 the main loop, 1.29
-// PFLOP/s), dx 432, dw 459, dh 84; [53000 x 128] [3920 x 128]^T fp32: 384, 317 and 350 us.
+// Measured (medians of 60 calls), [8192 x 4096] [8192 x 4096]^T bf16 with gelu and a residual: forward 540 us (425 the
+// main loop, 1.29 PFLOP/s), dx 434, dw 459, dh 93; [53000 x 128] [3920 x 128]^T fp32: 387, 321 and 344 us.
 #include "elements.hpp"
 
 #include <math.h>
@@ -41,7 +41,7 @@ enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5 }
 
 // FAST (16-bit results): reciprocals and exponentials of the hardware's precision, and Phi(h) from a fit of
 // log(erfc(z) e^(z^2) / t) by a polynomial in t = 1 / (1 + 0.3 z) on 0 <= z <= 9.5 (least squares, reweighted to an
-// even error of 4.3e-7): gelu is off by 2e-7 at most, a hundredth of half a step of fp16 near 0.01, and
+// even error of 4.3e-7): gelu is off by 2e-7 at most, a twentieth of half a step of fp16 near 0.01, and
 // costs 14 instructions where erff, both of whose branches a wave takes, costs 50 (the 8192 x 8192 forward
 // with it spent 300 us of 820 in the epilogue).
 template <bool FAST>

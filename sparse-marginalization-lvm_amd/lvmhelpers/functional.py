@@ -267,7 +267,8 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     GPU; residual has exactly the output's shape (nothing is broadcast).  activation: 'none', 'relu', 'gelu' (the erf
     form), 'silu', 'sigmoid', 'tanh'.  Products are summed in fp32; float32 operands are multiplied to
     fp32 accuracy on the bf16 matrix cores (an infinite operand may then give NaN instead of an
-    infinity).  Differentiable in all four; `bias`' gradient comes from the pass that computes `weight`'s."""
+    infinity).  Differentiable in all four, once and in reverse mode; `bias`' gradient comes from the pass that
+    applies the activation's slope, without an activation from the one that computes `weight`'s."""
     name = "linear_act"
     act = _native.ACTIVATIONS.get(activation)
     if act is None:

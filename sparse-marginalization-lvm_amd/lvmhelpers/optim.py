@@ -2,8 +2,9 @@
 
 No counterpart in the reference, whose scripts use torch's optimisers.  A step of a small model is
 launch bound (the batch-64 models of `bench_models.py` have 10 to 20 parameter tensors); here the
-whole update of up to 40 tensors is one kernel of csrc/adamw.hip, step counters included, and
-nothing is read back, so it runs unchanged inside `lvmhelpers.graphs.GraphedStep`.
+whole update of up to 40 tensors is one kernel of csrc/adamw.hip, step counters included (captured, and for
+large models, they are a second, small one), and nothing is read back, so it runs unchanged inside
+`lvmhelpers.graphs.GraphedStep`.
 
     opt = AdamW(model.parameters(), lr=1e-3)
     step = GraphedStep(model, opt, first_batch)
@@ -21,7 +22,6 @@ from . import _native
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _STATE_32 = ("exp_avg", "exp_avg_sq")
-_STATE_8 = ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale")
 BLOCK = 256     # elements that share one scale of an 8-bit state
 
 
