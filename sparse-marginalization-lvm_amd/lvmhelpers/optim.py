@@ -55,6 +55,8 @@ class AdamW(torch.optim.Optimizer):
         self._order = {p: i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
         self.__dict__.setdefault("_tickets", {})
         self.__dict__.setdefault("_captured", False)
+        if "_loading" in self.__dict__:
+            self._load(*self.__dict__.pop("_loading"))
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -125,6 +127,15 @@ class AdamW(torch.optim.Optimizer):
         into the tensors of the states and of a tensor `lr` that are there already (a number that is loaded
         for a tensor lr fills it).  Once a step has been captured, a state that state_dict does not have
         starts anew in its own memory, and one of another kind (32 for 8 bits) is refused."""
+        # (a hook behind the caller's own sees the dict that is loaded; __setstate__ runs before the hooks that follow)
+        handle = self.register_load_state_dict_pre_hook(AdamW._before_load)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            handle.remove()
+            self.__dict__.pop("_loading", None)
+
+    def _before_load(self, state_dict):
         held = {p: dict(st) for p, st in self.state.items()}
         rates = [g["lr"] for g in self.param_groups]
         loaded = {p: state_dict["state"].get(i, {}) for g, saved in zip(self.param_groups, state_dict["param_groups"])
@@ -138,11 +149,13 @@ class AdamW(torch.optim.Optimizer):
         for rate, saved in zip(rates, state_dict["param_groups"]):
             if torch.is_tensor(rate) and float(first.setdefault(id(rate), saved["lr"])) != float(saved["lr"]):
                 raise ValueError("AdamW.load_state_dict: groups that share one tensor lr would get different rates")
-        super().load_state_dict(state_dict)
+        self._loading = held, rates, loaded
+
+    @torch.no_grad()
+    def _load(self, held, rates, loaded):
         for group, rate in zip(self.param_groups, rates):
             if torch.is_tensor(rate):
-                with torch.no_grad():
-                    rate.copy_(group["lr"]) if torch.is_tensor(group["lr"]) else rate.fill_(group["lr"])
+                rate.copy_(group["lr"]) if torch.is_tensor(group["lr"]) else rate.fill_(group["lr"])
                 group["lr"] = rate
         for p, st in loaded.items():
             if self._captured and held.get(p) and not st:

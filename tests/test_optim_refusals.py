@@ -170,3 +170,27 @@ def test_a_parameter_twice_in_a_group_is_refused():
     with pytest.raises(ValueError):
         opt.add_param_group({"params": [p, p]})
     assert len(opt.param_groups) == 1
+
+
+def test_load_state_dict_hooks_see_and_change_what_is_loaded(not_capturing):
+    """A hook's own dict is what is loaded, states included, and hooks that run afterwards see them as they stay."""
+    opt, p = _with_state(bits=8)
+    other, _ = _with_state(bits=8)
+
+    def doubled(opt, sd):
+        state = {i: {k: torch.full_like(v, 2) for k, v in st.items()} for i, st in sd["state"].items()}
+        return {"state": state, "param_groups": [dict(g, lr=0.125) for g in sd["param_groups"]]}
+    seen = {}
+    opt.register_load_state_dict_pre_hook(doubled)
+    opt.register_load_state_dict_post_hook(lambda o: seen.update({k: (v.dtype, v.clone()) for k, v in o.state[p].items()}))
+    opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.125 and len(opt._optimizer_load_state_dict_pre_hooks) == 1
+    for k, v in opt.state[p].items():
+        assert bool((v.float() == 2).all()) and seen[k][0] == v.dtype == other.state_dict()["state"][0][k].dtype
+        assert torch.equal(seen[k][1].float(), v.float())
+    opt._captured = True
+    number, _ = _with_state(bits=32)
+    opt.register_load_state_dict_pre_hook(lambda o, sd: number.state_dict())
+    with pytest.raises(ValueError):                 # what the hook makes of it is what is checked
+        opt.load_state_dict(other.state_dict())
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == 2 and bool((opt.state[p]["exp_rms"].float() == 2).all())
